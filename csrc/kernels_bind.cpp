@@ -15,6 +15,7 @@ long long launch_count() { return g_launches.load(std::memory_order_relaxed); }
 
 void register_ep_comm(pybind11::module& m);
 void register_elementwise(pybind11::module& m);
+void register_losses(pybind11::module& m);
 
 namespace {
 void trace_stamp(at::Tensor& ring, at::Tensor& counter, int64_t tag) {
@@ -35,4 +36,5 @@ void register_kernels(pybind11::module& m) {
   m.def("trace_stamp", &trace_stamp, "append (tag, device time) to a device timeline ring");
   register_ep_comm(m);
   register_elementwise(m);
+  register_losses(m);
 }

@@ -1,0 +1,351 @@
+// Python bindings of the vocabulary losses (vocab_loss.cu) and of the router with a balance
+// loss (router_balance.cu).
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <cmath>
+#include <string>
+
+#include "router_balance.h"
+#include "vocab_loss.h"
+
+namespace {
+
+// Numbers go into messages through std::to_string: the stream insertion of an integer
+// crashes where the extension's C++ runtime differs from the interpreter's.
+
+// The last of an entry point's checks, so that the others speak on any machine.
+void need_cuda(const at::Tensor& t, const char* name) { TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor"); }
+
+cudaStream_t cs() { return at::cuda::getCurrentCUDAStream().stream(); }
+int sms() { return at::cuda::getCurrentDeviceProperties()->multiProcessorCount; }
+
+int vocab_dtype(const at::Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return sepx::kVocabBf16;
+    case at::kHalf: return sepx::kVocabF16;
+    case at::kFloat: return sepx::kVocabF32;
+    default: TORCH_CHECK(false, name, " must be bf16, fp16 or fp32, not ", t.scalar_type());
+  }
+}
+
+void req_rows(const at::Tensor& t, const at::Tensor& z, const char* name) {
+  TORCH_CHECK(t.device() == z.device(), name, " must be on the logits' device");
+  TORCH_CHECK(t.dim() == 1 && t.size(0) == z.size(0), name, " must be [", std::to_string(z.size(0)), "]");
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+}
+void req_f32_rows(const at::Tensor& t, const at::Tensor& z, const char* name) {
+  req_rows(t, z, name);
+  TORCH_CHECK(t.scalar_type() == at::kFloat, name, " must be fp32");
+}
+bool ids_are_64(const at::Tensor& t, const char* name) {
+  TORCH_CHECK(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64");
+  return t.scalar_type() == at::kLong;
+}
+
+// Common part: logits, gradient buffer and temperature.
+sepx::VocabLossArgs vocab_args(const at::Tensor& z, const c10::optional<at::Tensor>& grad, double tau) {
+  TORCH_CHECK(z.dim() == 2, "logits must be [T, V]");
+  TORCH_CHECK(z.size(1) >= 1 && z.size(1) <= 0x7fffff00, "logits must have a vocabulary of 1 to 2^31 - 256 columns");
+  TORCH_CHECK(z.size(0) <= 0x7fffffff / 8, "too many rows");
+  TORCH_CHECK(z.stride(1) == 1 || z.size(1) == 1, "logits must have unit stride along the vocabulary");
+  TORCH_CHECK(std::isfinite(tau) && tau > 0, "temperature must be positive and finite");
+  sepx::VocabLossArgs a;
+  a.z = z.data_ptr();
+  a.z_stride = z.stride(0);
+  a.dtype = vocab_dtype(z, "logits");
+  a.T = (int)z.size(0);
+  a.V = (int)z.size(1);
+  a.c2 = (float)(1.4426950408889634 / tau);
+  TORCH_CHECK(std::isfinite(a.c2) && a.c2 > 0, "temperature out of range");
+  a.tau = (float)tau;
+  if (grad.has_value()) {
+    TORCH_CHECK(grad->device() == z.device() && grad->scalar_type() == z.scalar_type() && grad->sizes() == z.sizes(),
+                "the gradient buffer must be like the logits");
+    TORCH_CHECK(grad->is_contiguous(), "the gradient buffer must be contiguous");
+    a.grad = grad->data_ptr();
+    a.grad_stride = grad->size(1);
+  }
+  return a;
+}
+
+void set_upstream(sepx::VocabLossArgs& a, const c10::optional<at::Tensor>& up, const at::Tensor& z) {
+  if (!up.has_value()) return;
+  TORCH_CHECK(up->device() == z.device() && up->numel() == 1 && up->scalar_type() == at::kFloat,
+              "the gradient of the loss must be one fp32 on the logits' device");
+  a.up = up->data_ptr<float>();
+}
+
+// num_valid >= 0: the rows in the loss, known on the host; negative: counted on the device.
+at::Tensor set_rows(sepx::VocabLossArgs& a, int op, int64_t num_valid, const at::Tensor& z) {
+  at::Tensor count;
+  if (num_valid >= 0) {
+    a.host_scale = 1.f / (float)std::max<int64_t>(num_valid, 1);
+  } else {
+    count = at::zeros({1}, z.options().dtype(at::kInt));
+    a.count = count.data_ptr<int>();
+    sepx::vocab_count_rows(a, op, count.data_ptr<int>(), cs());
+  }
+  return count;
+}
+
+// Returns the loss; the gradient (of the loss times `up`) goes to `grad`, which may be the
+// logits themselves.
+at::Tensor distill_loss(const at::Tensor& z, const at::Tensor& ids, const at::Tensor& teacher, double tau,
+                        int64_t num_valid, const c10::optional<at::Tensor>& grad, const c10::optional<at::Tensor>& up) {
+  auto a = vocab_args(z, grad, tau);
+  TORCH_CHECK(ids.device() == z.device() && teacher.device() == z.device(),
+              "teacher ids and logits must be on the logits' device");
+  TORCH_CHECK(ids.dim() == 2 && ids.size(0) == z.size(0), "teacher_ids must be [", std::to_string(z.size(0)), ", K]");
+  TORCH_CHECK(teacher.sizes() == ids.sizes(), "teacher_logits must have the shape of teacher_ids");
+  TORCH_CHECK(ids.size(1) >= 1 && ids.size(1) <= sepx::kMaxTeacher, "a row has 1 to ", std::to_string(sepx::kMaxTeacher),
+              " teacher entries, not ", std::to_string(ids.size(1)));
+  TORCH_CHECK(ids.is_contiguous() && teacher.is_contiguous(), "teacher_ids and teacher_logits must be contiguous");
+  TORCH_CHECK(teacher.scalar_type() == at::kFloat, "teacher_logits must be fp32");
+  a.ids64 = ids_are_64(ids, "teacher_ids");
+  need_cuda(z, "logits");
+  const c10::cuda::CUDAGuard guard(z.device());
+  a.ids = ids.data_ptr();
+  a.teacher = teacher.data_ptr<float>();
+  a.K = (int)ids.size(1);
+  set_upstream(a, up, z);
+  const auto f32 = z.options().dtype(at::kFloat);
+  at::Tensor loss = at::empty({}, f32), rows = at::empty({a.T}, f32);
+  const at::Tensor count = set_rows(a, sepx::kOpDistill, num_valid, z);
+  a.row_loss = rows.data_ptr<float>();
+  sepx::vocab_loss(a, sepx::kOpDistill, cs());
+  sepx::vocab_loss_sum(a, loss.data_ptr<float>(), cs());
+  return loss;
+}
+
+// Returns (loss, logp [T], kl [T]).
+std::vector<at::Tensor> policy_loss(const at::Tensor& z, const at::Tensor& actions, const at::Tensor& old_logp,
+                                    const at::Tensor& advantages, const c10::optional<at::Tensor>& ref_logp,
+                                    double clip_low, double clip_high, double kl_coef, double tau, int64_t num_valid,
+                                    const c10::optional<at::Tensor>& grad, const c10::optional<at::Tensor>& up) {
+  auto a = vocab_args(z, grad, tau);
+  req_rows(actions, z, "actions");
+  req_f32_rows(old_logp, z, "old_logp");
+  req_f32_rows(advantages, z, "advantages");
+  if (ref_logp.has_value()) req_f32_rows(*ref_logp, z, "ref_logp");
+  TORCH_CHECK(clip_low >= 0 && clip_low <= 1 && clip_high >= 0, "clip_low must be in [0, 1], clip_high >= 0");
+  TORCH_CHECK(std::isfinite(kl_coef) && kl_coef >= 0, "kl_coef must be finite and >= 0");
+  TORCH_CHECK(kl_coef == 0 || ref_logp.has_value(), "a KL term needs ref_logp");
+  a.ids64 = ids_are_64(actions, "actions");
+  need_cuda(z, "logits");
+  const c10::cuda::CUDAGuard guard(z.device());
+  a.labels = actions.data_ptr();
+  a.old_logp = old_logp.data_ptr<float>();
+  a.adv = advantages.data_ptr<float>();
+  a.ref_logp = ref_logp.has_value() ? ref_logp->data_ptr<float>() : nullptr;
+  a.clip_low = (float)clip_low;
+  a.clip_high = (float)clip_high;
+  a.kl_coef = (float)kl_coef;
+  set_upstream(a, up, z);
+  const auto f32 = z.options().dtype(at::kFloat);
+  at::Tensor loss = at::empty({}, f32), rows = at::empty({a.T}, f32);
+  at::Tensor logp = at::empty({a.T}, f32), kl = at::empty({a.T}, f32);
+  const at::Tensor count = set_rows(a, sepx::kOpPolicy, num_valid, z);
+  a.row_loss = rows.data_ptr<float>();
+  a.logp = logp.data_ptr<float>();
+  a.kl = kl.data_ptr<float>();
+  sepx::vocab_loss(a, sepx::kOpPolicy, cs());
+  sepx::vocab_loss_sum(a, loss.data_ptr<float>(), cs());
+  return {loss, logp, kl};
+}
+
+// Log-probability [T] of each row's label.
+at::Tensor token_logp(const at::Tensor& z, const at::Tensor& labels, double tau) {
+  auto a = vocab_args(z, c10::nullopt, tau);
+  req_rows(labels, z, "labels");
+  a.ids64 = ids_are_64(labels, "labels");
+  need_cuda(z, "logits");
+  const c10::cuda::CUDAGuard guard(z.device());
+  a.labels = labels.data_ptr();
+  at::Tensor logp = at::empty({a.T}, z.options().dtype(at::kFloat));
+  a.logp = logp.data_ptr<float>();
+  sepx::vocab_loss(a, sepx::kOpLogp, cs());
+  return logp;
+}
+
+void set_offsets(sepx::VocabLossArgs& a, const at::Tensor& offsets, const at::Tensor& z) {
+  TORCH_CHECK(offsets.device() == z.device() && offsets.scalar_type() == at::kInt && offsets.is_contiguous() &&
+                  offsets.dim() == 1 && offsets.size(0) % 2 == 1,
+              "seq_offsets must be a contiguous int32 vector of 2 * pairs + 1 entries on the logits' device");
+  a.offsets = offsets.data_ptr<int>();
+  a.num_seq = (int)offsets.size(0) - 1;
+}
+
+// Returns (loss, rewards [2 * pairs], logp [T], lse [T, 2], row_coef [T] = d loss / d logp).
+// With `grad` (may be the logits), d logp / d logits of each row is written there, negated.
+std::vector<at::Tensor> preference_fwd(const at::Tensor& z, const at::Tensor& labels, const at::Tensor& offsets,
+                                       const at::Tensor& ref_logp, double beta, double eps,
+                                       const c10::optional<at::Tensor>& grad) {
+  auto a = vocab_args(z, grad, 1.0);
+  req_rows(labels, z, "labels");
+  req_f32_rows(ref_logp, z, "ref_logp");
+  set_offsets(a, offsets, z);
+  TORCH_CHECK(std::isfinite(beta) && beta > 0, "beta must be positive and finite");
+  TORCH_CHECK(eps >= 0 && eps < 0.5, "label_smoothing must be in [0, 0.5)");
+  a.ids64 = ids_are_64(labels, "labels");
+  need_cuda(z, "logits");
+  const c10::cuda::CUDAGuard guard(z.device());
+  a.labels = labels.data_ptr();
+  const auto f32 = z.options().dtype(at::kFloat);
+  at::Tensor logp = at::empty({a.T}, f32), lse = at::empty({a.T, 2}, f32);
+  a.logp = logp.data_ptr<float>();
+  a.lse = lse.data_ptr<float>();
+  sepx::vocab_loss(a, sepx::kOpLogp, cs());
+
+  sepx::PreferenceArgs q;
+  q.logp = a.logp;
+  q.ref_logp = ref_logp.data_ptr<float>();
+  q.labels = a.labels;
+  q.ids64 = a.ids64;
+  q.offsets = a.offsets;
+  q.T = a.T;
+  q.pairs = a.num_seq / 2;
+  q.beta = (float)beta;
+  q.eps = (float)eps;
+  at::Tensor loss = at::empty({}, f32), rewards = at::empty({2 * (int64_t)q.pairs}, f32);
+  at::Tensor pair_loss = at::empty({q.pairs}, f32), row_coef = at::zeros({a.T}, f32);
+  q.rewards = rewards.data_ptr<float>();
+  q.pair_loss = pair_loss.data_ptr<float>();
+  q.row_coef = row_coef.data_ptr<float>();
+  sepx::preference_pairs(q, cs());
+  sepx::preference_loss_sum(q.pair_loss, q.pairs, loss.data_ptr<float>(), cs());
+  return {loss, rewards, logp, lse, row_coef};
+}
+
+// d (up * loss) / d logits from the forward's lse and row_coef.
+at::Tensor preference_grad(const at::Tensor& z, const at::Tensor& labels, const at::Tensor& offsets,
+                           const at::Tensor& lse, const at::Tensor& row_coef, const at::Tensor& up) {
+  at::Tensor grad = at::empty(z.sizes(), z.options().memory_format(at::MemoryFormat::Contiguous));
+  auto a = vocab_args(z, grad, 1.0);
+  req_rows(labels, z, "labels");
+  req_f32_rows(row_coef, z, "row_coef");
+  TORCH_CHECK(lse.device() == z.device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
+                  lse.numel() == 2 * z.size(0),
+              "lse must be [T, 2] fp32");
+  set_offsets(a, offsets, z);
+  need_cuda(z, "logits");
+  const c10::cuda::CUDAGuard guard(z.device());
+  a.labels = labels.data_ptr();
+  a.ids64 = ids_are_64(labels, "labels");
+  a.lse = lse.data_ptr<float>();
+  set_upstream(a, up, z);
+  sepx::preference_grad(a, row_coef.data_ptr<float>(), cs());
+  return grad;
+}
+
+// grad *= up in place (nothing is read where up is 1).
+void scale_grad(at::Tensor& grad, const at::Tensor& up) {
+  TORCH_CHECK(grad.is_contiguous(), "grad must be contiguous");
+  TORCH_CHECK(up.device() == grad.device() && up.numel() == 1 && up.scalar_type() == at::kFloat,
+              "the gradient of the loss must be one fp32 on the same device");
+  need_cuda(grad, "grad");
+  const c10::cuda::CUDAGuard guard(grad.device());
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(grad.data_ptr()) % 16 == 0, "grad must be 16-byte aligned");
+  sepx::vocab_scale_grad(grad.data_ptr(), vocab_dtype(grad, "grad"), grad.numel(), up.data_ptr<float>(), sms(), cs());
+}
+
+sepx::RouterBalanceArgs router_args(const at::Tensor& x, int64_t k, bool renorm, const c10::optional<at::Tensor>& valid) {
+  TORCH_CHECK(x.dim() == 2 && x.size(0) <= 0x7fffffff / 32, "router logits must be [T, E]");
+  const int64_t E = x.size(1);
+  TORCH_CHECK(E >= 1 && E <= sepx::kRouterMaxExperts, "1 to ", std::to_string(sepx::kRouterMaxExperts),
+              " experts, not ", std::to_string(E));
+  TORCH_CHECK(k >= 1 && k <= sepx::kRouterMaxK && k <= E, "k must be 1 to min(",
+              std::to_string(sepx::kRouterMaxK), ", experts), not ", std::to_string(k));
+  TORCH_CHECK(x.stride(1) == 1 || E == 1, "router logits must have unit stride along the experts");
+  sepx::RouterBalanceArgs a;
+  a.x = x.data_ptr();
+  a.x_stride = x.stride(0);
+  a.dtype = vocab_dtype(x, "router logits");
+  a.T = (int)x.size(0);
+  a.E = (int)E;
+  a.k = (int)k;
+  a.renorm = renorm;
+  if (valid.has_value()) {
+    TORCH_CHECK(valid->device() == x.device() && valid->scalar_type() == at::kBool && valid->is_contiguous() &&
+                    valid->dim() == 1 && valid->size(0) == x.size(0),
+                "valid must be a contiguous bool vector, one entry per token, on the logits' device");
+    a.valid = reinterpret_cast<const uint8_t*>(valid->data_ptr<bool>());
+  }
+  return a;
+}
+
+// Returns (topk_w [T, k], topk_e [T, k] int32, loss, counts [E] int32, coef [E]).
+std::vector<at::Tensor> router_balance_fwd(const at::Tensor& x, int64_t k, bool renorm,
+                                           const c10::optional<at::Tensor>& bias,
+                                           const c10::optional<at::Tensor>& valid) {
+  auto a = router_args(x, k, renorm, valid);
+  if (bias.has_value()) {
+    TORCH_CHECK(bias->device() == x.device() && bias->scalar_type() == at::kFloat && bias->is_contiguous() &&
+                    bias->dim() == 1 && bias->size(0) == x.size(1),
+                "bias must be a contiguous fp32 vector, one entry per expert, on the logits' device");
+    a.bias = bias->data_ptr<float>();
+  }
+  need_cuda(x, "router logits");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const auto f32 = x.options().dtype(at::kFloat), i32 = x.options().dtype(at::kInt);
+  a.blocks = sepx::router_balance_blocks(a.T, sms());
+  at::Tensor w = at::empty({a.T, a.k}, f32), e = at::empty({a.T, a.k}, i32);
+  at::Tensor loss = at::empty({}, f32), counts = at::empty({a.E}, i32), coef = at::empty({a.E}, f32);
+  at::Tensor part = at::empty({a.blocks, 2 * (int64_t)a.E + 1}, f32);
+  a.topk_w = w.data_ptr<float>();
+  a.topk_e = e.data_ptr<int>();
+  a.loss = loss.data_ptr<float>();
+  a.counts = counts.data_ptr<int>();
+  a.coef = coef.data_ptr<float>();
+  a.part_p = part.data_ptr<float>();
+  a.part_c = reinterpret_cast<int*>(a.part_p + (int64_t)a.blocks * a.E);
+  a.part_n = a.part_c + (int64_t)a.blocks * a.E;
+  sepx::router_balance_fwd(a, cs());
+  return {w, e, loss, counts, coef};
+}
+
+// d logits from the gradients of topk_w and of the loss (either may be absent).
+at::Tensor router_balance_bwd(const at::Tensor& x, const at::Tensor& topk_e, const at::Tensor& coef, bool renorm,
+                              const c10::optional<at::Tensor>& valid, const c10::optional<at::Tensor>& dw,
+                              const c10::optional<at::Tensor>& dloss) {
+  TORCH_CHECK(topk_e.dim() == 2 && topk_e.scalar_type() == at::kInt && topk_e.is_contiguous() &&
+                  topk_e.device() == x.device() && topk_e.size(0) == x.size(0),
+              "topk_e must be the forward's");
+  auto a = router_args(x, topk_e.size(1), renorm, valid);
+  TORCH_CHECK(coef.device() == x.device() && coef.scalar_type() == at::kFloat && coef.is_contiguous() &&
+                  coef.numel() == x.size(1),
+              "coef must be the forward's");
+  if (dw.has_value()) {
+    TORCH_CHECK(dw->device() == x.device() && dw->scalar_type() == at::kFloat && dw->is_contiguous() &&
+                    dw->sizes() == topk_e.sizes(),
+                "dw must be a contiguous fp32 tensor of topk_w's shape");
+    a.dw = dw->data_ptr<float>();
+  }
+  if (dloss.has_value()) {
+    TORCH_CHECK(dloss->device() == x.device() && dloss->scalar_type() == at::kFloat && dloss->numel() == 1,
+                "the gradient of the loss must be one fp32 on the logits' device");
+    a.dloss = dloss->data_ptr<float>();
+  }
+  need_cuda(x, "router logits");
+  const c10::cuda::CUDAGuard guard(x.device());
+  at::Tensor dx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  a.topk_e = topk_e.data_ptr<int>();
+  a.coef = coef.data_ptr<float>();
+  a.dx = dx.data_ptr();
+  sepx::router_balance_bwd(a, sms(), cs());
+  return dx;
+}
+
+}  // namespace
+
+void register_losses(pybind11::module& m) {
+  m.def("distill_loss", &distill_loss);
+  m.def("policy_loss", &policy_loss);
+  m.def("token_logp", &token_logp);
+  m.def("preference_fwd", &preference_fwd);
+  m.def("preference_grad", &preference_grad);
+  m.def("scale_grad", &scale_grad);
+  m.def("router_balance_fwd", &router_balance_fwd);
+  m.def("router_balance_bwd", &router_balance_bwd);
+}

@@ -1,0 +1,76 @@
+// Losses over a vocabulary's logits and the balanced router: launch parameters and
+// launchers (vocab_loss.cu, router_balance.cu).
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace sepx {
+
+enum VocabDtype : int { kVocabBf16 = 0, kVocabF16 = 1, kVocabF32 = 2 };
+enum VocabOp : int {
+  kOpDistill = 0,  // soft targets: a teacher's top logits
+  kOpPolicy = 1,   // one chosen token per row, clipped ratio loss with a KL term
+  kOpLogp = 2,     // one token per row: its log-probability (and the unit gradient)
+};
+
+constexpr int kMaxTeacher = 1024;  // teacher entries per row
+
+struct VocabLossArgs {
+  const void* z = nullptr;  // [T, V] logits, unit column stride
+  int64_t z_stride = 0;     // elements between rows
+  void* grad = nullptr;     // [T, V] gradient, may be z; null: loss only
+  int64_t grad_stride = 0;
+  int dtype = kVocabBf16;
+  int T = 0, V = 0;
+  float c2 = 0.f;            // log2(e) / temperature
+  float tau = 1.f;           // temperature
+  float host_scale = 1.f;    // 1 / rows in the loss, when the host knows it ...
+  const int* count = nullptr;  // ... else the number of rows, on the device
+  const float* up = nullptr;   // optional gradient of the loss, on the device
+  // kOpDistill
+  const void* ids = nullptr;  // [T, K] int32 / int64; negative: no entry
+  const float* teacher = nullptr;  // [T, K] logits
+  int K = 0;
+  // kOpPolicy / kOpLogp
+  const void* labels = nullptr;  // [T] int32 / int64; negative: row not in the loss
+  bool ids64 = false;            // ids / labels are int64
+  const float* old_logp = nullptr;
+  const float* adv = nullptr;
+  const float* ref_logp = nullptr;  // may be null (no KL term)
+  float clip_low = 0.f, clip_high = 0.f, kl_coef = 0.f;
+  const int* offsets = nullptr;  // kOpLogp: rows outside [offsets[0], offsets[num_seq]) are not in the loss
+  int num_seq = 0;
+  // outputs, [T] fp32
+  float* row_loss = nullptr;  // kOpDistill / kOpPolicy
+  float* logp = nullptr;      // kOpPolicy / kOpLogp
+  float* kl = nullptr;        // kOpPolicy
+  float* lse = nullptr;       // kOpLogp: [T, 2], the row's maximum and log2 of sum 2^((z - max) c2)
+};
+
+// Rows in the loss: *count = number of rows with a label >= 0 (labels [T]), or with a
+// teacher entry (ids / teacher [T, K]). count must be zero before the call.
+void vocab_count_rows(const VocabLossArgs& a, int op, int* count, cudaStream_t st);
+void vocab_loss(const VocabLossArgs& a, int op, cudaStream_t st);
+// *loss = sum(row_loss[0..T)) / rows (host_scale or count), in a fixed order.
+void vocab_loss_sum(const VocabLossArgs& a, float* loss, cudaStream_t st);
+// grad *= *up, in place; nothing is touched where *up is 1.
+void vocab_scale_grad(void* grad, int dtype, int64_t n, const float* up, int num_sms, cudaStream_t st);
+
+struct PreferenceArgs {
+  const float* logp = nullptr;   // [T]
+  const float* ref_logp = nullptr;  // [T]
+  const void* labels = nullptr;  // [T]
+  bool ids64 = false;
+  const int* offsets = nullptr;  // [2 * pairs + 1]
+  int T = 0, pairs = 0;
+  float beta = 0.f, eps = 0.f;
+  float* rewards = nullptr;    // [2 * pairs]
+  float* pair_loss = nullptr;  // [pairs]
+  float* row_coef = nullptr;   // [T] d loss / d logp, zero-filled before the call
+};
+void preference_pairs(const PreferenceArgs& a, cudaStream_t st);
+void preference_loss_sum(const float* pair_loss, int pairs, float* loss, cudaStream_t st);
+// grad[t] = up * row_coef[t] * (onehot(labels[t]) - softmax(z[t])), zeros where row_coef is 0.
+void preference_grad(const VocabLossArgs& a, const float* row_coef, cudaStream_t st);
+
+}  // namespace sepx

@@ -4,10 +4,22 @@ The logits GEMM and both gradient GEMMs run on the tcgen05 GEMM (``spec_ep.ops.l
 the vocabulary's last 256-column tile is partial); the softmax cross-entropy and its
 gradient run in one sm_100a kernel that overwrites the bf16 logits with
 ``(softmax - onehot) * scale`` so no fp32 copy of the [T, V] logits is ever stored.
+
+Three objectives for training after the pre-training, on the kernels of
+csrc/vocab_loss.cu, each over given logits and as an ``lm_head_*`` form that owns the
+logits and overwrites them with their gradient:
+
+* ``topk_distill_loss``: distillation from a teacher's top logits,
+* ``clipped_policy_loss``: clipped policy ratio with a KL term to a reference model,
+* ``preference_loss``: paired log-ratios of packed chosen / rejected sequences
+  (``token_logp`` gives the reference model's side, and a rollout's).
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._ext import load
 from .linear import dense_dgrad, dense_fwd, dense_wgrad
@@ -53,3 +65,187 @@ def lm_head_xent(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, num_val
 def lm_head_xent_reference(h, w, labels):
     logits = h.float() @ w.float().t()
     return torch.nn.functional.cross_entropy(logits, labels.long(), ignore_index=-1)
+
+
+# ----------------------------------------------------------------------------------------
+# losses after pre-training
+# ----------------------------------------------------------------------------------------
+def _valid(num_valid):
+    """Rows in the loss for the kernels: -1 counts them on the device."""
+    if num_valid is None:
+        return -1
+    if num_valid < 0:
+        raise ValueError(f"num_valid must be >= 0, not {num_valid}")
+    return int(num_valid)
+
+
+def _wants_grad(logits):
+    return torch.is_grad_enabled() and logits.requires_grad
+
+
+def _hand_over(ctx, up, again):
+    """Gradient of the logits for upstream ``up``. The forward formed it in its pass over
+    the logits; it is handed out once, scaled in place (not touched where ``up`` is 1). A
+    second backward through the same graph, or fp16 logits, whose unscaled gradient could
+    leave the type's range, compute it from the logits."""
+    grad, ctx.grad = ctx.grad, None
+    up = up.contiguous()
+    if grad is None:
+        return again(up)
+    load().scale_grad(grad, up)
+    return grad
+
+
+class _TopkDistill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, teacher, tau, num_valid, want):
+        ctx.grad = logits.new_empty(logits.shape) if want and logits.dtype != torch.float16 else None
+        loss = load().distill_loss(logits, ids, teacher, tau, num_valid, ctx.grad, None)
+        ctx.save_for_backward(logits, ids, teacher)
+        ctx.cfg = (tau, num_valid)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, up):
+        logits, ids, teacher = ctx.saved_tensors
+        tau, num_valid = ctx.cfg
+
+        def again(up):
+            grad = logits.new_empty(logits.shape)
+            load().distill_loss(logits, ids, teacher, tau, num_valid, grad, up)
+            return grad
+
+        return _hand_over(ctx, up, again), None, None, None, None, None
+
+
+def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+                      temperature: float = 1.0, num_valid: int | None = None) -> torch.Tensor:
+    """Distillation from a teacher's top logits: mean over rows of
+    ``temperature^2 * KL(p || q)``, ``p`` the softmax of the row's listed teacher logits and
+    ``q`` the softmax of all its ``logits``, both over ``temperature``.
+
+    ``logits [T, V]`` bf16, fp16 or fp32 (any row stride); ``teacher_ids [T, K]`` int32 or
+    int64 and ``teacher_logits [T, K]``, ``K <= 1024``. An id below 0, or a teacher logit of
+    -inf, is no entry (what stands beside such an id is not looked at); a row without
+    entries is not in the loss, its logits are not read and its gradient is 0. The same id
+    twice counts with both weights. An id outside the vocabulary makes the loss NaN.
+    ``num_valid`` (rows with an entry, if the host knows it) spares a count on the device.
+    Gradients reach ``logits`` only.
+    """
+    return _TopkDistill.apply(logits, teacher_ids.contiguous(), teacher_logits.detach().float().contiguous(),
+                              float(temperature), _valid(num_valid), _wants_grad(logits))
+
+
+class PolicyLoss(NamedTuple):
+    loss: torch.Tensor  # scalar
+    logp: torch.Tensor  # [T] log-probability of each action (0 where there is none)
+    kl: torch.Tensor    # [T] estimate of the KL to the reference model (0 without one)
+
+
+class _ClippedPolicy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, actions, old_logp, advantages, ref_logp, cfg, want):
+        ctx.grad = logits.new_empty(logits.shape) if want and logits.dtype != torch.float16 else None
+        loss, logp, kl = load().policy_loss(logits, actions, old_logp, advantages, ref_logp, cfg[0], cfg[1], cfg[2],
+                                            cfg[3], cfg[4], ctx.grad, None)
+        ctx.save_for_backward(logits, actions, old_logp, advantages, ref_logp)
+        ctx.cfg = cfg
+        ctx.mark_non_differentiable(logp, kl)
+        ctx.set_materialize_grads(False)
+        return loss, logp, kl
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, up, _dlogp, _dkl):
+        if up is None:
+            return None, None, None, None, None, None, None
+        logits, actions, old_logp, advantages, ref_logp = ctx.saved_tensors
+        cfg = ctx.cfg
+
+        def again(up):
+            grad = logits.new_empty(logits.shape)
+            load().policy_loss(logits, actions, old_logp, advantages, ref_logp, cfg[0], cfg[1], cfg[2], cfg[3],
+                               cfg[4], grad, up)
+            return grad
+
+        return _hand_over(ctx, up, again), None, None, None, None, None, None
+
+
+def _f32_rows(t):
+    return None if t is None else t.detach().float().contiguous()
+
+
+def clipped_policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logp: torch.Tensor,
+                        advantages: torch.Tensor, ref_logp: torch.Tensor | None = None, clip_low: float = 0.2,
+                        clip_high: float = 0.2, kl_coef: float = 0.0, temperature: float = 1.0,
+                        num_valid: int | None = None) -> PolicyLoss:
+    """Clipped policy loss over tokens, with a KL term to a reference model.
+
+    With ``logp`` the log-probability of the row's action under
+    ``softmax(logits / temperature)`` and ``r = exp(logp - old_logp)``::
+
+        loss = mean( -min(r * A, clip(r, 1 - clip_low, 1 + clip_high) * A)
+                     + kl_coef * (exp(d) - d - 1) ),   d = ref_logp - logp
+
+    The mean is over rows with an action; an action below 0 leaves its row (a prompt token)
+    out: the row is not read and its gradient is 0. ``logits [T, V]`` bf16, fp16 or fp32
+    (any row stride), ``actions [T]`` int32 or int64, the others ``[T]``. An action outside
+    the vocabulary makes the loss NaN. ``num_valid`` (rows with an action, if the host
+    knows it) spares a count on the device. Gradients reach ``logits`` only.
+    """
+    cfg = (float(clip_low), float(clip_high), float(kl_coef), float(temperature), _valid(num_valid))
+    return PolicyLoss(*_ClippedPolicy.apply(logits, actions.contiguous(), _f32_rows(old_logp), _f32_rows(advantages),
+                                            _f32_rows(ref_logp), cfg, _wants_grad(logits)))
+
+
+def token_logp(logits: torch.Tensor, labels: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
+    """Log-probability ``[T]`` (fp32) of each row's label under ``softmax(logits /
+    temperature)``, 0 where the label is below 0. No gradient: the ``old_logp`` and
+    ``ref_logp`` of the losses here."""
+    return load().token_logp(logits.detach(), labels.contiguous(), float(temperature))
+
+
+class PreferenceLoss(NamedTuple):
+    loss: torch.Tensor     # scalar
+    rewards: torch.Tensor  # [2 * pairs] beta * (sum of logp - ref_logp) of each sequence
+    logp: torch.Tensor     # [T] log-probability of each label (0 where there is none)
+
+
+class _Preference(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, offsets, ref_logp, beta, eps):
+        loss, rewards, logp, lse, coef = load().preference_fwd(logits, labels, offsets, ref_logp, beta, eps, None)
+        ctx.save_for_backward(logits, labels, offsets, lse, coef)
+        ctx.mark_non_differentiable(rewards, logp)
+        ctx.set_materialize_grads(False)
+        return loss, rewards, logp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, up, _drewards, _dlogp):
+        if up is None:
+            return None, None, None, None, None, None
+        logits, labels, offsets, lse, coef = ctx.saved_tensors
+        grad = load().preference_grad(logits, labels, offsets, lse, coef, up.contiguous())
+        return grad, None, None, None, None, None
+
+
+def preference_loss(logits: torch.Tensor, labels: torch.Tensor, seq_offsets: torch.Tensor, ref_logp: torch.Tensor,
+                    beta: float = 0.1, label_smoothing: float = 0.0) -> PreferenceLoss:
+    """Paired preference loss over packed sequences: sequence ``s`` is the rows
+    ``seq_offsets[s] .. seq_offsets[s + 1]``, sequence ``2 i`` the chosen and ``2 i + 1`` the
+    rejected one of pair ``i``. With ``R_s = beta * sum(logp - ref_logp)`` over its labels::
+
+        m_i  = R_2i - R_2i+1
+        loss = mean_i( -(1 - eps) * log sigmoid(m_i) - eps * log sigmoid(-m_i) )
+
+    ``logits [T, V]`` bf16, fp16 or fp32 (any row stride), ``labels [T]`` int32 or int64
+    (below 0: not in the loss, as a prompt's tokens), ``ref_logp [T]`` the reference model's
+    log-probabilities of the same labels (``token_logp``), ``seq_offsets [2 * pairs + 1]``
+    int32, not decreasing. Rows outside all sequences, and rows without a label, are not
+    read and their gradient is 0. A label outside the vocabulary makes the loss NaN.
+    Gradients reach ``logits`` only.
+    """
+    return PreferenceLoss(*_Preference.apply(logits, labels.contiguous(), seq_offsets.contiguous(),
+                                             _f32_rows(ref_logp), float(beta), float(label_smoothing)))
