@@ -60,6 +60,7 @@ sepx::VocabLossArgs vocab_args(const at::Tensor& z, const c10::optional<at::Tens
   a.c2 = (float)(1.4426950408889634 / tau);
   TORCH_CHECK(std::isfinite(a.c2) && a.c2 > 0, "temperature out of range");
   a.tau = (float)tau;
+  a.tau64 = tau;
   if (grad.has_value()) {
     TORCH_CHECK(grad->device() == z.device() && grad->scalar_type() == z.scalar_type() && grad->sizes() == z.sizes(),
                 "the gradient buffer must be like the logits");
@@ -90,6 +91,17 @@ at::Tensor set_rows(sepx::VocabLossArgs& a, int op, int64_t num_valid, const at:
   return count;
 }
 
+// Scratch of a call: records, partial sums and a ticket in one allocation.
+at::Tensor set_scratch(sepx::VocabLossArgs& a, const at::Tensor& z) {
+  const int64_t rec = (int64_t)a.T * sepx::kRowRecordBytes, part = (int64_t)sepx::vocab_finish_blocks(a.T) * 8;
+  at::Tensor s = at::empty({rec + part + 16}, z.options().dtype(at::kByte));
+  uint8_t* p = s.data_ptr<uint8_t>();
+  a.records = p;
+  a.partial = reinterpret_cast<double*>(p + rec);
+  a.ticket = reinterpret_cast<unsigned int*>(p + rec + part);
+  return s;
+}
+
 // Returns the loss; the gradient (of the loss times `up`) goes to `grad`, which may be the
 // logits themselves.
 at::Tensor distill_loss(const at::Tensor& z, const at::Tensor& ids, const at::Tensor& teacher, double tau,
@@ -111,11 +123,10 @@ at::Tensor distill_loss(const at::Tensor& z, const at::Tensor& ids, const at::Te
   a.K = (int)ids.size(1);
   set_upstream(a, up, z);
   const auto f32 = z.options().dtype(at::kFloat);
-  at::Tensor loss = at::empty({}, f32), rows = at::empty({a.T}, f32);
-  const at::Tensor count = set_rows(a, sepx::kOpDistill, num_valid, z);
-  a.row_loss = rows.data_ptr<float>();
-  sepx::vocab_loss(a, sepx::kOpDistill, cs());
-  sepx::vocab_loss_sum(a, loss.data_ptr<float>(), cs());
+  at::Tensor loss = at::empty({}, f32);
+  const at::Tensor count = set_rows(a, sepx::kOpDistill, num_valid, z), scratch = set_scratch(a, z);
+  a.loss = loss.data_ptr<float>();
+  sepx::vocab_loss(a, sepx::kOpDistill, sms(), cs());
   return loss;
 }
 
@@ -144,14 +155,12 @@ std::vector<at::Tensor> policy_loss(const at::Tensor& z, const at::Tensor& actio
   a.kl_coef = (float)kl_coef;
   set_upstream(a, up, z);
   const auto f32 = z.options().dtype(at::kFloat);
-  at::Tensor loss = at::empty({}, f32), rows = at::empty({a.T}, f32);
-  at::Tensor logp = at::empty({a.T}, f32), kl = at::empty({a.T}, f32);
-  const at::Tensor count = set_rows(a, sepx::kOpPolicy, num_valid, z);
-  a.row_loss = rows.data_ptr<float>();
+  at::Tensor loss = at::empty({}, f32), logp = at::empty({a.T}, f32), kl = at::empty({a.T}, f32);
+  const at::Tensor count = set_rows(a, sepx::kOpPolicy, num_valid, z), scratch = set_scratch(a, z);
+  a.loss = loss.data_ptr<float>();
   a.logp = logp.data_ptr<float>();
   a.kl = kl.data_ptr<float>();
-  sepx::vocab_loss(a, sepx::kOpPolicy, cs());
-  sepx::vocab_loss_sum(a, loss.data_ptr<float>(), cs());
+  sepx::vocab_loss(a, sepx::kOpPolicy, sms(), cs());
   return {loss, logp, kl};
 }
 
@@ -165,7 +174,8 @@ at::Tensor token_logp(const at::Tensor& z, const at::Tensor& labels, double tau)
   a.labels = labels.data_ptr();
   at::Tensor logp = at::empty({a.T}, z.options().dtype(at::kFloat));
   a.logp = logp.data_ptr<float>();
-  sepx::vocab_loss(a, sepx::kOpLogp, cs());
+  const at::Tensor scratch = set_scratch(a, z);
+  sepx::vocab_loss(a, sepx::kOpLogp, sms(), cs());
   return logp;
 }
 
@@ -195,12 +205,15 @@ std::vector<at::Tensor> preference_fwd(const at::Tensor& z, const at::Tensor& la
   const auto f32 = z.options().dtype(at::kFloat);
   at::Tensor logp = at::empty({a.T}, f32), lse = at::empty({a.T, 2}, f32);
   a.logp = logp.data_ptr<float>();
+  at::Tensor ratio = at::empty({a.T}, f32);
   a.lse = lse.data_ptr<float>();
-  sepx::vocab_loss(a, sepx::kOpLogp, cs());
+  a.ref_logp = ref_logp.data_ptr<float>();
+  a.ratio = ratio.data_ptr<float>();
+  const at::Tensor scratch = set_scratch(a, z);
+  sepx::vocab_loss(a, sepx::kOpLogp, sms(), cs());
 
   sepx::PreferenceArgs q;
-  q.logp = a.logp;
-  q.ref_logp = ref_logp.data_ptr<float>();
+  q.ratio = a.ratio;
   q.labels = a.labels;
   q.ids64 = a.ids64;
   q.offsets = a.offsets;

@@ -312,6 +312,13 @@ __device__ __forceinline__ uint32_t mapa_shared(uint32_t a, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Two floats to a shared::cluster address, counted (8 bytes) on the mbarrier at the
+// shared::cluster address `bar` of the same CTA.
+__device__ __forceinline__ void st_async_f2(uint32_t to, float a, float b, uint32_t bar) {
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(to), "f"(a),
+               "f"(b), "r"(bar)
+               : "memory");
+}
 // arrive on an mbarrier given by its shared::cluster address (this or the peer CTA)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");

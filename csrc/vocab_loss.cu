@@ -6,25 +6,25 @@
 //                  dz = -(1 / tau) dloss/dl (q - onehot(a))
 //   log-prob       l = ln softmax(z)[y] for the preference loss
 // All three need the row's log-sum-exp and one gradient form, A (q - P) with a P of few
-// entries, so one kernel body serves them. Exponentials are 2^((z - max) c2) with
-// c2 = log2(e) / tau: the difference first, so a row of the type's lowest or highest values
-// does not overflow on the way. Logits are read as they are (bf16, fp16 or fp32), everything
-// is computed in fp32, and the gradient is rounded once, to the logits' type.
+// entries, so one kernel body serves them. Logits are read as they are (bf16, fp16 or fp32),
+// everything is computed in fp32, and the gradient is rounded once, to the logits' type.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <array>
+#include <map>
+#include <mutex>
 #include <stdexcept>
 #include <string>
 
 #include "kernels.h"
+#include "sm100.cuh"
 #include "vocab_loss.h"
 
 namespace sepx {
 namespace {
-
-constexpr float kLn2 = 0.69314718055994531f;
 
 void check_launch(const char* what) {
   note_launch();
@@ -37,10 +37,10 @@ __device__ __forceinline__ float warp_sum(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
+__device__ __forceinline__ float warp_max(float v) {  // NaN gives way
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
 __device__ __forceinline__ float block_sum(float v, float* s) {  // s: 32 floats
   v = warp_sum(v);
@@ -59,11 +59,55 @@ __device__ __forceinline__ float block_max(float v, float* s) {
   return warp_max((int)(threadIdx.x & 31) < nw ? s[threadIdx.x & 31] : -INFINITY);
 }
 
+__device__ __forceinline__ double block_sum_d(double v, double* s) {  // s: 32 doubles
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+  __syncthreads();
+  const int nw = blockDim.x >> 5;
+  v = (int)(threadIdx.x & 31) < nw ? s[threadIdx.x & 31] : 0.0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
 // 2^x, hardware approximation (results below 2^-126 flush to 0: nothing beside a sum >= 1)
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two floats in one 64-bit register: sm_100 does one multiply-add for both.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(F2 a, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(a.v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 ex2_2(F2 a) {
+  float x, y;
+  split(a, x, y);
+  return f2(ex2(x), ex2(y));
 }
 
 // ------------------------------------------------------------------------------------
@@ -172,167 +216,290 @@ __device__ __forceinline__ int64_t load_id(const void* p, int64_t i, bool is64) 
 }
 
 // ------------------------------------------------------------------------------------
-// The sparse side of a row: its entries in shared memory, K of them (1 for a token)
+// Exponentials of a row: 2^(z c2 - M2), c2 = log2(e) / tau, M2 = the rounded product m c2 of
+// a reference m (the row's maximum, or near it). The same rounded M2 enters the sum, the
+// gradient and the logarithm, so its rounding cancels. Where m c2 leaves fp32 (rows whose
+// largest value is the type's lowest or highest), the difference z - m comes first.
 // ------------------------------------------------------------------------------------
-struct Entries {
-  int* id;    // -1: not an entry
-  float* p;   // weight P; where ids repeat, the gradient takes the sum of their weights
-  float* lp;  // ln P (distillation)
-  float* z;   // the row's logit at id
+constexpr float kFarM2 = 1e37f;
+struct Expo {
+  float c2, m, M2;
+  bool far;
+  __device__ __forceinline__ Expo(float c2_, float m_) {
+    c2 = c2_;
+    m = m_;
+    M2 = __fmul_rn(m_, c2_);
+    far = !(fabsf(M2) <= kFarM2);
+  }
+  __device__ __forceinline__ float arg(float z) const { return far ? (z - m) * c2 : fmaf(z, c2, -M2); }
+  __device__ __forceinline__ float operator()(float z) const { return ex2(arg(z)); }
+  // a sum against reference r, against this reference instead
+  __device__ __forceinline__ float join(float r, float s) const {
+    if (r == -INFINITY) return s;  // nothing yet: 0 (or NaN, which stays)
+    return s * ex2(far ? (r - m) * c2 : __fmul_rn(r, c2) - M2);
+  }
 };
-__host__ __device__ inline size_t entries_bytes(int op, int K) { return op == kOpDistill ? (size_t)K * 16 : 16; }
-__device__ __forceinline__ Entries entries_at(void* smem, int K) {
-  float* f = reinterpret_cast<float*>(smem);
-  return {reinterpret_cast<int*>(f), f + K, f + 2 * K, f + 3 * K};
+
+// Largest element of a vector and ref; NaN gives way.
+template <typename T>
+__device__ __forceinline__ float max_of(const uint4& raw, float ref) {
+  float o[Elem<T>::N];
+  Elem<T>::unpack(raw, o);
+#pragma unroll
+  for (int i = 0; i < Elem<T>::N; ++i) ref = fmaxf(ref, o[i]);
+  return ref;
+}
+// What the fast form z c2 + R adds for reference m: NaN (or infinity) where the sum has to
+// take the careful form.
+__device__ __forceinline__ float reference(float m, float c2) {
+  const Expo w(c2, m);
+  return m == -INFINITY ? INFINITY : w.far ? __int_as_float(0x7fffffff) : -w.M2;
 }
 
+// The careful forms of the two passes over n vectors `step` apart in shared memory: a sum
+// whose reference moves, and a gradient with another phase, at a row's ends, or of a row
+// with a far reference. Out of line: they are rare, and inline they cost the usual path.
+template <typename T>
+__device__ __noinline__ float2 careful_sum(const uint4* v, int n, int step, float c2, float ref, float sum) {
+  float m = ref;
+  for (int k = 0; k < n; ++k) m = max_of<T>(v[k * step], m);
+  const Expo w(c2, m == -INFINITY ? 0.f : m);
+  sum = w.join(ref, sum);
+  for (int k = 0; k < n; ++k) {
+    float o[Elem<T>::N];
+    Elem<T>::unpack(v[k * step], o);
+#pragma unroll
+    for (int i = 0; i < Elem<T>::N; ++i) sum += w(o[i]);
+  }
+  return make_float2(m, sum);
+}
+template <typename T>
+__device__ __noinline__ void careful_store(const uint4* v, int n, int step, T* row, int V, int64_t e0, float c2, float m,
+                                           float As) {
+  constexpr int N = Elem<T>::N;
+  const Expo w(c2, m);
+  const RowVec<T> g(row, V);
+  for (int k = 0; k < n; ++k) {
+    float o[N];
+    Elem<T>::unpack(v[k * step], o);
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = As * w(o[i]);
+    g.store(e0 + (int64_t)k * step * N, o);
+  }
+}
+__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort, nullptr, 2000000000ull)) != 0;
+}
+
+// ------------------------------------------------------------------------------------
+// The sparse side of a row. One token per row (policy, log-probability) or K entries of a
+// teacher in shared memory (distillation). What a row's outputs need is left in a RowRecord;
+// a second kernel forms the outputs of all rows at once, in 64 bits.
+// ------------------------------------------------------------------------------------
 // A row's part in the loss. Bad: an id outside the vocabulary, which turns the row's
 // outputs into NaN (and is never used as an index).
 enum RowState : int { kRowOff = 0, kRowOn = 1, kRowBad = 2 };
 
-// Fills id / p / lp of row t; called by all threads, which all get the row's state.
-template <int OP>
-__device__ __forceinline__ int row_entries(const VocabLossArgs& a, int t, const Entries& s, float* red) {
-  if constexpr (OP == kOpDistill) {
-    float top = -INFINITY;
-    int any = 0, bad = 0;
-    for (int k = threadIdx.x; k < a.K; k += blockDim.x) {
-      const int64_t id = load_id(a.ids, (int64_t)t * a.K + k, a.ids64);
-      const float v = a.teacher[(int64_t)t * a.K + k];
-      const bool has = id >= 0 && v != -INFINITY;
-      any |= has;
-      bad |= has && id >= a.V;
-      s.id[k] = has ? (int)(id < a.V ? id : 0) : -1;
-      s.p[k] = v;
-      if (has) top = fmaxf(top, v);
-    }
-    any = __syncthreads_or(any);
-    bad = __syncthreads_or(bad);
-    if (!any) return kRowOff;
-    top = block_max(top, red);
-    float sum = 0.f;
-    for (int k = threadIdx.x; k < a.K; k += blockDim.x)
-      if (s.id[k] >= 0) sum += expf((s.p[k] - top) / a.tau);
-    sum = block_sum(sum, red);
-    const float lsum = logf(sum);
-    for (int k = threadIdx.x; k < a.K; k += blockDim.x) {
-      const bool has = s.id[k] >= 0;
-      const float lp = has ? (s.p[k] - top) / a.tau - lsum : 0.f;
-      s.lp[k] = lp;
-      s.p[k] = has ? expf(lp) : 0.f;
-    }
-    __syncthreads();
-    return bad ? kRowBad : kRowOn;
-  } else {
-    const int64_t id = load_id(a.labels, t, a.ids64);
-    bool on = id >= 0;
-    if (OP == kOpLogp && a.offsets) on = on && t >= a.offsets[0] && t < a.offsets[a.num_seq];
-    if (threadIdx.x == 0) {
-      s.id[0] = on && id < a.V ? (int)id : (on ? 0 : -1);
-      s.p[0] = 1.f;
-    }
-    __syncthreads();
-    return !on ? kRowOff : id < a.V ? kRowOn : kRowBad;
+struct RowRecord {
+  double base;    // distillation: sum P ln P - sum P (z - zref) c2 ln 2
+  float m, sum;   // the row's reference and sum of exponentials
+  float z;        // the token's logit; distillation: zref
+  float weight;   // distillation: sum P
+  int state;
+  int pad;
+};
+static_assert(sizeof(RowRecord) == kRowRecordBytes, "scratch size");
+
+struct Entries {
+  int* id;    // -1: not an entry
+  float* p;   // weight, after the teacher's logit
+  float* z;   // the row's logit at id
+  int K4;     // entries, up to a multiple of 4 (those past K are none)
+};
+constexpr int kEntryBytes = 12;
+__host__ __device__ inline int entries_padded(int K) { return (K + 3) / 4 * 4; }
+__device__ __forceinline__ Entries entries_at(void* smem, int K) {
+  const int K4 = entries_padded(K);
+  float* f = reinterpret_cast<float*>(smem);
+  return {reinterpret_cast<int*>(f), f + K4, f + 2 * K4, K4};
+}
+// The weight at an id: the sum over all entries with it, in their order (so equal ids get
+// the same bits).
+__device__ __forceinline__ float weight_of(const Entries& s, int id) {
+  float P = 0.f;
+  for (int j = 0; j < s.K4; j += 4) {
+    const int4 i = *reinterpret_cast<const int4*>(s.id + j);
+    const float4 p = *reinterpret_cast<const float4*>(s.p + j);
+    P += i.x == id ? p.x : 0.f;
+    P += i.y == id ? p.y : 0.f;
+    P += i.z == id ? p.z : 0.f;
+    P += i.w == id ? p.w : 0.f;
   }
+  return P;
 }
 
-// 1 / rows in the loss
-__device__ __forceinline__ float rows_scale(const VocabLossArgs& a) {
-  return a.count ? 1.f / (float)max(*a.count, 1) : a.host_scale;
-}
+// What the gradient takes from one token (policy, log-probability).
+struct Token {
+  int state, id;
+  float z, adv, old_logp, ref_logp;  // z: its logit
+};
 
-// Outputs of a row that is not in the loss (one thread).
-template <int OP>
-__device__ __forceinline__ void row_off(const VocabLossArgs& a, int t) {
-  if (OP != kOpLogp) a.row_loss[t] = 0.f;
-  if (OP != kOpDistill) a.logp[t] = 0.f;
-  if (OP == kOpPolicy) a.kl[t] = 0.f;
-  if (OP == kOpLogp && a.lse) reinterpret_cast<float2*>(a.lse)[t] = make_float2(0.f, 0.f);
-}
-
-// Outputs of a row in the loss (from the threads of the block that has `write`), and the
-// factor A of its gradient A (q - P) (all threads). mx = the row's maximum, l2s = log2 of
-// sum 2^((z - mx) c2).
-template <int OP>
-__device__ __forceinline__ float row_on(const VocabLossArgs& a, int t, int state, const Entries& s, float mx, float l2s,
-                                        float* red, bool write) {
-  const float nan = __int_as_float(0x7fffffff);
-  if constexpr (OP == kOpDistill) {
-    if (write) {
-      float d = 0.f;
-      for (int k = threadIdx.x; k < a.K; k += blockDim.x)
-        if (s.id[k] >= 0 && s.p[k] != 0.f) d += s.p[k] * (s.lp[k] - kLn2 * fmaf(s.z[k] - mx, a.c2, -l2s));
-      d = block_sum(d, red);
-      if (threadIdx.x == 0) a.row_loss[t] = state == kRowBad ? nan : a.tau * a.tau * d;
-    }
-    if (state == kRowBad) return nan;
-    return a.tau * rows_scale(a) * (a.up ? *a.up : 1.f);
-  } else {
-    const float logp = state == kRowBad ? nan : kLn2 * fmaf(s.z[0] - mx, a.c2, -l2s);
-    if constexpr (OP == kOpLogp) {
-      if (write && threadIdx.x == 0) {
-        a.logp[t] = logp;
-        if (a.lse) reinterpret_cast<float2*>(a.lse)[t] = make_float2(mx, l2s);
-      }
-      return -1.f;
-    } else {
-      const float A = a.adv[t], r = expf(logp - a.old_logp[t]);
-      // an advantage of 0 asks for nothing, also where the ratio overflows
-      const float u = A == 0.f ? 0.f : r * A;
-      const float v = A == 0.f ? 0.f : fminf(fmaxf(r, 1.f - a.clip_low), 1.f + a.clip_high) * A;
-      float loss = -(u <= v ? u : v), dl = u <= v ? -u : 0.f, kl = 0.f;
-      if (r != r) loss = dl = nan;  // the clamp drops NaN
-      if (a.ref_logp) {
-        const float d = a.ref_logp[t] - logp, em = expm1f(d);
-        kl = em - d;
-        if (a.kl_coef != 0.f) {
-          loss += a.kl_coef * kl;
-          dl -= a.kl_coef * em;
-        }
-      }
-      if (write && threadIdx.x == 0) {
-        a.row_loss[t] = loss;
-        a.logp[t] = logp;
-        a.kl[t] = kl;
-      }
-      return -dl / a.tau * rows_scale(a) * (a.up ? *a.up : 1.f);
+template <typename T, int OP>
+__device__ __forceinline__ Token load_token(const VocabLossArgs& a, int t, const T* row) {
+  const int64_t id = load_id(a.labels, t, a.ids64);
+  bool on = id >= 0;
+  if (OP == kOpLogp && a.offsets) on = on && t >= a.offsets[0] && t < a.offsets[a.num_seq];
+  Token k = {!on ? kRowOff : id < a.V ? kRowOn : kRowBad, 0, 0.f, 0.f, 0.f, 0.f};
+  if (on) {
+    k.id = k.state == kRowOn ? (int)id : 0;
+    k.z = Elem<T>::f(row[k.id]);
+    if constexpr (OP == kOpPolicy) {
+      k.adv = a.adv[t];
+      k.old_logp = a.old_logp[t];
+      k.ref_logp = a.ref_logp ? a.ref_logp[t] : 0.f;
     }
   }
+  return k;
 }
 
-// The weight at entry k's id: the sum over the entries with the same id, in their order.
+// Fills the teacher entries of row t from one warp and returns the row's state; lane 0 has
+// the record's sparse half in *rec.
+template <typename T>
+__device__ __forceinline__ int load_entries(const VocabLossArgs& a, int t, const T* row, const Entries& s, int lane,
+                                            RowRecord* rec) {
+  const int K = a.K;
+  float top = -INFINITY;
+  bool any = false, bad = false;
+  if (lane < s.K4 - K) {
+    s.id[K + lane] = -1;
+    s.p[K + lane] = 0.f;
+  }
+  for (int k = lane; k < K; k += 32) {
+    const int64_t id = load_id(a.ids, (int64_t)t * K + k, a.ids64);
+    const float v = a.teacher[(int64_t)t * K + k];
+    const bool has = id >= 0 && v != -INFINITY;
+    any |= has;
+    bad |= has && id >= a.V;
+    s.id[k] = has ? (int)(id < a.V ? id : 0) : -1;
+    s.p[k] = v;
+    if (has) top = fmaxf(top, v);
+  }
+  if (!__any_sync(0xffffffffu, any)) return rec->state = kRowOff;
+  bad = __any_sync(0xffffffffu, bad);
+  top = warp_max(top);
+  float sum = 0.f, zref = -INFINITY;
+  for (int k = lane; k < K; k += 32) {
+    const int id = s.id[k];
+    const float z = id >= 0 ? Elem<T>::f(row[id]) : 0.f;
+    s.z[k] = z;
+    if (id >= 0) {
+      sum += expf((s.p[k] - top) / a.tau);
+      zref = fmaxf(zref, z);
+    }
+  }
+  const float lsum = logf(warp_sum(sum));
+  zref = warp_max(zref);
+  if (zref == -INFINITY) zref = 0.f;
+  double base = 0.0;
+  float weight = 0.f;
+  for (int k = lane; k < K; k += 32) {
+    const bool has = s.id[k] >= 0;
+    const float lp = has ? (s.p[k] - top) / a.tau - lsum : 0.f;
+    const float P = has ? expf(lp) : 0.f;
+    s.p[k] = P;
+    if (P != 0.f) {  // P (ln P - (z - zref) / tau): the logits' exponent as the sum has it
+      base += (double)P * ((double)lp - ((double)s.z[k] - (double)zref) * ((double)a.c2 * 0.69314718055994530942));
+      weight += P;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) base += __shfl_xor_sync(0xffffffffu, base, o);
+  rec->base = base;
+  rec->weight = warp_sum(weight);
+  rec->z = zref;
+  rec->state = bad ? kRowBad : kRowOn;
+  __syncwarp();
+  return rec->state;
+}
+
+// The policy loss of one token from r = pi / pi_old and d = ln (pi_ref / pi).
+struct PolicyTerm {
+  float loss, dl, kl;  // dl = d loss / d logp
+};
+__device__ __forceinline__ PolicyTerm policy_term(const VocabLossArgs& a, float A, float r, float d, bool has_ref) {
+  // an advantage of 0 asks for nothing, also where the ratio overflows
+  const float u = A == 0.f ? 0.f : r * A;
+  const float v = A == 0.f ? 0.f : fminf(fmaxf(r, 1.f - a.clip_low), 1.f + a.clip_high) * A;
+  PolicyTerm o;
+  o.loss = -(u <= v ? u : v);
+  o.dl = u <= v ? -u : 0.f;
+  o.kl = 0.f;
+  if (r != r) o.loss = o.dl = r;  // the clamp drops NaN
+  if (has_ref) {
+    const float em = expm1f(d);
+    o.kl = em - d;
+    if (a.kl_coef != 0.f) {
+      o.loss += a.kl_coef * o.kl;
+      o.dl -= a.kl_coef * em;
+    }
+  }
+  return o;
+}
+
+// d (up * loss) / d (sum over rows)
+__device__ __forceinline__ float loss_factor(const VocabLossArgs& a) {
+  return (a.count ? 1.f / (float)max(*a.count, 1) : a.host_scale) * (a.up ? *a.up : 1.f);
+}
+
+// The factor A of the gradient A (q - P) of a row in the loss. x: the row's exponentials,
+// sum: theirs; g: loss_factor.
 template <int OP>
-__device__ __forceinline__ float weight_at(const Entries& s, int K, int k) {
-  if (OP != kOpDistill) return 1.f;
-  const int id = s.id[k];
-  float p = 0.f;
-  for (int j = 0; j < K; ++j)
-    if (s.id[j] == id) p += s.p[j];
-  return p;
+__device__ __forceinline__ float row_factor(const VocabLossArgs& a, const Token& k, const Expo& x, float sum, float g) {
+  if (k.state == kRowBad) return __int_as_float(0x7fffffff);
+  if constexpr (OP == kOpLogp) return -1.f;
+  if constexpr (OP == kOpDistill) return a.tau * g;
+  const float lp = x.arg(k.z) * 0.69314718055994531f - logf(sum);
+  return -policy_term(a, k.adv, expf(lp - k.old_logp), k.ref_logp - lp, a.ref_logp != nullptr).dl / a.tau * g;
 }
 
-// One block per row, any vocabulary: the row is read for its maximum, and again (from L2
-// where it fits) for the sum and for the gradient.
+// Rows longer than a cluster's shared memory: one block per row, which reads the row for its
+// maximum, and again (from L2 where it fits) for the sum and for the gradient.
 template <typename T, int OP>
 __global__ void __launch_bounds__(512) vocab_row_kernel(const VocabLossArgs a) {
   constexpr int N = Elem<T>::N;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float red[32];
-  const int t = blockIdx.x;
-  const int K = OP == kOpDistill ? a.K : 1;
-  const Entries s = entries_at(smem, K);
+  __shared__ Token s_token;
+  const int t = blockIdx.x, lane = threadIdx.x & 31;
+  const Entries s = entries_at(smem, a.K);
   const RowVec<T> z(const_cast<T*>(reinterpret_cast<const T*>(a.z)) + (int64_t)t * a.z_stride, a.V);
   const RowVec<T> g(reinterpret_cast<T*>(a.grad) + (a.grad ? (int64_t)t * a.grad_stride : 0), a.V);
-  const int state = row_entries<OP>(a, t, s, red);
-  if (state == kRowOff) {
-    if (threadIdx.x == 0) row_off<OP>(a, t);
+  RowRecord* rec = reinterpret_cast<RowRecord*>(a.records) + t;
+  if (threadIdx.x < 32) {
+    RowRecord r = {};
+    Token k = {};
+    if constexpr (OP == kOpDistill) {
+      k.state = load_entries(a, t, z.p, s, lane, &r);
+    } else {
+      k = load_token<T, OP>(a, t, z.p);
+      r.z = k.z;
+      r.state = k.state;
+    }
+    if (lane == 0) {
+      s_token = k;
+      *rec = r;
+      if (t == 0) *a.ticket = 0;
+    }
+  }
+  __syncthreads();
+  const Token k = s_token;
+  if (k.state == kRowOff) {
     if (a.grad) {
       const float o[N] = {};
-      for (int j = threadIdx.x; j < g.nv; j += blockDim.x) g.store(g.first(j), o);
+      for (int j = threadIdx.x; j < z.nv; j += blockDim.x) g.store(z.first(j), o);
     }
     return;
   }
-  for (int k = threadIdx.x; k < K; k += blockDim.x) s.z[k] = s.id[k] >= 0 ? Elem<T>::f(z.p[s.id[k]]) : 0.f;
   float mx = -INFINITY, sum = 0.f;
   for (int j = threadIdx.x; j < z.nv; j += blockDim.x) {
     float o[N];
@@ -340,29 +507,487 @@ __global__ void __launch_bounds__(512) vocab_row_kernel(const VocabLossArgs a) {
 #pragma unroll
     for (int i = 0; i < N; ++i) mx = fmaxf(mx, o[i]);
   }
-  mx = block_max(mx, red);
+  const Expo x(a.c2, block_max(mx, red));
   for (int j = threadIdx.x; j < z.nv; j += blockDim.x) {
     float o[N];
     Elem<T>::unpack(z.load(j), o);
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum += ex2((o[i] - mx) * a.c2);
+    for (int i = 0; i < N; ++i) sum += x(o[i]);
   }
   sum = block_sum(sum, red);
-  const float l2s = log2f(sum);
-  __syncthreads();  // s.z
-  const float A = row_on<OP>(a, t, state, s, mx, l2s, red, true);
+  if (threadIdx.x == 0) {
+    rec->m = x.m;
+    rec->sum = sum;
+  }
   if (!a.grad) return;
-  __syncthreads();
+  const float A = row_factor<OP>(a, k, x, sum, loss_factor(a)), As = A / sum;
   for (int j = threadIdx.x; j < z.nv; j += blockDim.x) {
     float o[N];
     Elem<T>::unpack(z.load(j), o);
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = A * ex2(fmaf(o[i] - mx, a.c2, -l2s));
+    for (int i = 0; i < N; ++i) o[i] = As * x(o[i]);
     g.store(z.first(j), o);
   }
   __syncthreads();
-  for (int k = threadIdx.x; k < K; k += blockDim.x)
-    if (s.id[k] >= 0) g.p[s.id[k]] = Elem<T>::t(A * (ex2(fmaf(s.z[k] - mx, a.c2, -l2s)) - weight_at<OP>(s, K, k)));
+  if constexpr (OP == kOpDistill) {
+    for (int i = threadIdx.x; i < a.K; i += blockDim.x)
+      if (s.id[i] >= 0) g.p[s.id[i]] = Elem<T>::t(As * x(s.z[i]) - A * weight_of(s, s.id[i]));
+  } else {
+    if (threadIdx.x == 0) g.p[k.id] = Elem<T>::t(As * x(k.z) - A);
+  }
+}
+
+// ------------------------------------------------------------------------------------
+// Streaming kernel. A cluster of C blocks takes a row: each block streams its part of the row
+// once from memory into a ring of pieces in shared memory, forms the partial sum as the
+// pieces arrive, exchanges it with the other blocks, and writes the gradient from the pieces,
+// which frees them for the next row. So every logit is read from memory once, and loads,
+// arithmetic and stores of neighbouring rows overlap.
+//   first CW warps  sum and gradient: thread i owns vectors i, i + 32 CW, .. of every piece
+//   load warp       bulk copies of whole vectors; the partial vectors at a row's ends come
+//                   from the prepare warp
+//   prepare warp    tokens (8 rows at a time) or teacher entries of the rows to come
+//   fix warp        distillation: the gradient at the entries' ids, once the block's dense
+//                   part is written (a single token is set by the thread that owns its vector)
+// Partial sums travel as (reference, sum) pairs of each warp, with asynchronous stores that
+// complete on the receiver's mbarrier. Pair buffers alternate: a warp sends row r + 2 after it
+// has row r + 1 of every warp, and each of those left after its block had all of row r.
+// Every wait is bounded; one that runs out turns the call's outputs into NaN.
+// ------------------------------------------------------------------------------------
+constexpr int kMaxSlots = 32, kMaxCluster = 8, kMaxConsumers = 16;
+
+// CW consumer warps, VPT vectors per thread and piece, B blocks per SM
+template <int CW_, int VPT_, int B_>
+struct StreamCfg {
+  static constexpr int CW = CW_, VPT = VPT_, B = B_;
+  static constexpr int Threads = (CW + 3) * 32;
+  static constexpr int Lanes = CW * 32;  // vectors between a thread's own
+  static constexpr int PieceVecs = Lanes * VPT, PieceBytes = PieceVecs * 16;
+};
+
+constexpr int kTokens = 16;  // rows between the prepare warp and the others (tokens)
+
+struct StreamShared {
+  uint64_t full[kMaxSlots], empty[kMaxSlots];
+  uint64_t ent_full[kTokens], ent_done[kTokens], dense_done[kTokens];
+  uint64_t pairs_full[2];
+  uint4 edge[kTokens][2];  // a row's first and last vector, where they are partial
+  Token token[kTokens];
+  float factor[kTokens][4];  // A, A / sum, reference
+  float2 pairs[2][kMaxCluster * kMaxConsumers];
+  int abort;
+};
+
+// The row's reference and sum from all warps' pairs (one warp; the same bits in each).
+__device__ __forceinline__ void join_pairs(const float2* pairs, int n, float c2, int lane, float* m, float* sum) {
+  float mx = -INFINITY, v = 0.f;
+  for (int i = lane; i < n; i += 32) mx = fmaxf(mx, pairs[i].x);
+  mx = warp_max(mx);
+  const Expo x(c2, mx);
+  for (int i = lane; i < n; i += 32) v += x.join(pairs[i].x, pairs[i].y);
+  v = warp_sum(v);
+  // a row without a finite logit has no softmax
+  *sum = mx == -INFINITY ? __int_as_float(0x7fffffff) : v;
+  *m = mx;
+}
+
+template <typename T, int OP, typename Cfg>
+__global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(const VocabLossArgs a, int C, int slots,
+                                                                            int rows_ahead) {
+  constexpr int N = Elem<T>::N, CW = Cfg::CW, kPieceVecs = Cfg::PieceVecs, kPieceBytes = Cfg::PieceBytes;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ StreamShared sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* ent_mem = ring + (size_t)slots * kPieceBytes;
+  auto entries = [&](int e) { return entries_at(ent_mem + (size_t)e * entries_padded(a.K) * kEntryBytes, a.K); };
+  const int rank = (int)(blockIdx.x % (unsigned)C);
+  const int cluster = (int)(blockIdx.x / (unsigned)C), clusters = (int)(gridDim.x / (unsigned)C);
+  volatile int* abort = &sh.abort;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < slots; ++i) {
+      mbar_init(&sh.full[i], 1);
+      mbar_init(&sh.empty[i], CW);
+    }
+    for (int i = 0; i < rows_ahead; ++i) {
+      mbar_init(&sh.ent_full[i], 1);
+      // the load warp, and the last reader: the consumers, or the fix warp after them
+      mbar_init(&sh.ent_done[i], OP == kOpDistill ? 2 : CW + 1);
+      mbar_init(&sh.dense_done[i], CW);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(&sh.pairs_full[i], C == 1 ? CW : 1);
+    sh.abort = 0;
+    fence_barrier_init();
+    if (blockIdx.x == 0) *a.ticket = 0;  // for the kernel that forms the outputs
+  }
+  __syncthreads();
+  if (C > 1) cluster_sync();  // the other blocks' barriers are ready too
+  auto wait = [&](uint64_t* bar, int phase) {  // all lanes of a warp, with one answer
+    const bool now = __all_sync(0xffffffffu, mbar_try_wait(bar, (uint32_t)phase & 1u));
+    return now || wait_slow(bar, (uint32_t)phase & 1u, abort);
+  };
+  const int log2c = 31 - __clz(C);
+  // this block's vectors of row t
+  auto row_z = [&](int t) {
+    return RowVec<T>(const_cast<T*>(reinterpret_cast<const T*>(a.z)) + (int64_t)t * a.z_stride, a.V);
+  };
+  auto part = [&](const RowVec<T>& z, int* j0, int* j1) {
+    const int per = (z.nv + C - 1) >> log2c;  // C is a power of two
+    *j0 = min(rank * per, z.nv);
+    *j1 = min(*j0 + per, z.nv);
+  };
+  // position in the ring of rows: entry e, in its lap's phase
+  auto next_entry = [&](int& e, int& lap) {
+    if (++e == rows_ahead) {
+      e = 0;
+      lap ^= 1;
+    }
+  };
+
+  if (warp == CW) {
+    // ------------------------------- loads -------------------------------
+    int slot = 0, turn = 0, e = 0, lap = 0;
+    bool ok = true;
+    for (int t = cluster; t < a.T && ok; t += clusters) {
+      if (!wait(&sh.ent_full[e], lap)) break;
+      if (sh.token[e].state != kRowOff) {
+        const RowVec<T> z = row_z(t);
+        int j0, j1;
+        part(z, &j0, &j1);
+        const int f0 = z.full(0) ? 0 : 1, f1 = z.full(z.nv - 1) ? z.nv : z.nv - 1;  // whole vectors
+        for (int p = j0; p < j1; p += kPieceVecs) {
+          const int q = min(p + kPieceVecs, j1);
+          if (!wait(&sh.empty[slot], turn ^ 1)) { ok = false; break; }
+          if (lane == 0) {
+            uint4* dst = reinterpret_cast<uint4*>(ring + (size_t)slot * kPieceBytes);
+            const bool head = p < f0, tail = q > f1;
+            if (head) dst[0] = sh.edge[e][0];
+            if (tail && z.nv - 1 >= f0) dst[z.nv - 1 - p] = sh.edge[e][1];
+            if (head || tail) fence_proxy_async_smem();  // before a later bulk copy into the slot
+            const int b0 = max(p, f0), b1 = min(q, f1);
+            if (b1 > b0) {
+              mbar_arrive_expect_tx(&sh.full[slot], (uint32_t)(b1 - b0) * 16u);
+              bulk_load(dst + (b0 - p), z.p + z.first(b0), (uint32_t)(b1 - b0) * 16u, &sh.full[slot]);
+            } else {
+              mbar_arrive(&sh.full[slot]);
+            }
+          }
+          __syncwarp();
+          if (++slot == slots) {
+            slot = 0;
+            turn ^= 1;
+          }
+        }
+      }
+      if (lane == 0) mbar_arrive(&sh.ent_done[e]);
+      __syncwarp();
+      next_entry(e, lap);
+    }
+  } else if (warp == CW + 1) {
+    // ------------------------------ prepare ------------------------------
+    RowRecord* recs = reinterpret_cast<RowRecord*>(a.records);
+    if constexpr (OP == kOpDistill) {
+      int e = 0, lap = 0;
+      for (int t = cluster; t < a.T; t += clusters) {
+        const RowVec<T> z = row_z(t);
+        if (!wait(&sh.ent_done[e], lap ^ 1)) break;
+        const bool head = !z.full(0), tail = !z.full(z.nv - 1);
+        if (head || tail) {  // lanes 0..N-1: the first vector, 16..16+N-1: the last
+          const int64_t at = lane < 16 ? z.first(0) + lane : z.first(z.nv - 1) + (lane - 16);
+          const float v = (lane & 15) < N && at >= 0 && at < z.V ? Elem<T>::f(z.p[at]) : -INFINITY;
+          if ((lane & 15) < N) reinterpret_cast<T*>(&sh.edge[e][lane >> 4])[lane & 15] = Elem<T>::t(v);
+        }
+        RowRecord r = {};
+        const int state = load_entries(a, t, z.p, entries(e), lane, &r);
+        __syncwarp();
+        if (lane == 0) {
+          sh.token[e].state = state;
+          if (rank == 0) {  // not the consumer's half
+            recs[t].base = r.base;
+            recs[t].z = r.z;
+            recs[t].weight = r.weight;
+            recs[t].state = state;
+          }
+          mbar_arrive(&sh.ent_full[e]);
+        }
+        __syncwarp();
+        next_entry(e, lap);
+      }
+    } else {
+      // lane i takes row i of each group of 8; two groups alternate, so one is prepared
+      // while the other is worked on
+      for (int g0 = 0;; g0 += kTokens / 2) {
+        const int64_t t = (int64_t)cluster + (int64_t)(g0 + lane) * clusters;
+        const bool mine = lane < kTokens / 2 && t < a.T;
+        if (!__any_sync(0xffffffffu, mine)) break;
+        const int e = (g0 + lane) % kTokens;
+        bool ok = true;
+        if (mine) ok = mbar_wait_bounded(&sh.ent_done[e], (uint32_t)(((g0 + lane) / kTokens) & 1) ^ 1u, abort, nullptr, 2000000000ull);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        if (mine) {
+          const RowVec<T> z = row_z((int)t);
+          const Token k = load_token<T, OP>(a, (int)t, z.p);
+          if (k.state != kRowOff) {
+            if (!z.full(0)) sh.edge[e][0] = z.load(0);
+            if (!z.full(z.nv - 1)) sh.edge[e][1] = z.load(z.nv - 1);
+          }
+          sh.token[e] = k;
+          if (rank == 0) {
+            recs[t].z = k.z;
+            recs[t].state = k.state;
+          }
+          mbar_arrive(&sh.ent_full[e]);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == CW + 2) {
+    // -------------------------------- fix --------------------------------
+    if constexpr (OP == kOpDistill) {
+      int e = 0, lap = 0;
+      for (int t = cluster; t < a.T; t += clusters) {
+        if (!wait(&sh.dense_done[e], lap)) break;
+        if (a.grad && sh.token[e].state != kRowOff) {  // the entries' values replace the dense ones
+          const Expo x(a.c2, sh.factor[e][2]);
+          const float A = sh.factor[e][0], As = sh.factor[e][1];
+          const Entries s = entries(e);
+          const RowVec<T> z = row_z(t);
+          int j0, j1;
+          part(z, &j0, &j1);
+          const int64_t e0 = z.first(j0), e1 = z.first(j1);
+          T* g = reinterpret_cast<T*>(a.grad) + (int64_t)t * a.grad_stride;
+          for (int k = lane; k < a.K; k += 32)
+            if (s.id[k] >= 0 && s.id[k] >= e0 && s.id[k] < e1) g[s.id[k]] = Elem<T>::t(As * x(s.z[k]) - A * weight_of(s, s.id[k]));
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.ent_done[e]);
+        __syncwarp();
+        next_entry(e, lap);
+      }
+    }
+  } else {
+    // ---------------------------- sum and gradient ----------------------------
+    const int tid = threadIdx.x;
+    const float factor = loss_factor(a);
+    int slot = 0, turn = 0, x = 0, e = 0, lap = 0;
+    bool ok = true;
+    for (int t = cluster; t < a.T && ok; t += clusters) {
+      if (!wait(&sh.ent_full[e], lap)) break;
+      const Token token = sh.token[e];
+      const RowVec<T> z = row_z(t);
+      const RowVec<T> g(reinterpret_cast<T*>(a.grad) + (a.grad ? (int64_t)t * a.grad_stride : 0), a.V);
+      int j0, j1;
+      part(z, &j0, &j1);
+      if (token.state == kRowOff) {
+        if (a.grad) {
+          const float o[N] = {};
+          for (int j = j0 + tid; j < j1; j += Cfg::Lanes) g.store(z.first(j), o);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(OP == kOpDistill ? &sh.dense_done[e] : &sh.ent_done[e]);
+        next_entry(e, lap);
+        continue;
+      }
+      if (C > 1 && warp == 0 && lane == 0) mbar_arrive_expect_tx(&sh.pairs_full[x & 1], (uint32_t)(C * CW) * 8u);
+      const int slot0 = slot;
+      const int mine = (j1 - j0 - tid + Cfg::Lanes - 1) / Cfg::Lanes;  // this thread's vectors (or < 1)
+      // Sum against a reference that is the maximum of the thread's first vectors: the sum may
+      // grow to 2^40 before the reference is moved, which costs fp32 nothing, so the usual
+      // vector takes no maximum.
+      float ref = -INFINITY, sum = 0.f;
+      F2 nR2 = f2(0.f, 0.f);
+      const F2 cc = f2(a.c2, a.c2);
+      for (int left = mine, first = 1, end = j1 - j0; end > 0; left -= Cfg::VPT, first = 0, end -= kPieceVecs) {
+        if (!wait(&sh.full[slot], turn)) { ok = false; break; }
+        const uint4* piece = reinterpret_cast<const uint4*>(ring + (size_t)slot * kPieceBytes) + tid;
+        if (end >= kPieceVecs) {
+          uint4 raw[Cfg::VPT];
+#pragma unroll
+          for (int v = 0; v < Cfg::VPT; ++v) raw[v] = piece[v * Cfg::Lanes];
+          if (first) {
+#pragma unroll
+            for (int v = 0; v < Cfg::VPT; ++v) ref = max_of<T>(raw[v], ref);
+            const float R = reference(ref, a.c2);
+            nR2 = f2(R, R);
+          }
+          F2 acc[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+#pragma unroll
+          for (int v = 0; v < Cfg::VPT; ++v) {
+            float o[N];
+            Elem<T>::unpack(raw[v], o);
+#pragma unroll
+            for (int i = 0; i < N; i += 2) acc[(i >> 1) & 1] = add2(acc[(i >> 1) & 1], ex2_2(fma2(f2(o[i], o[i + 1]), cc, nR2)));
+          }
+          float ax, ay;
+          split(add2(acc[0], acc[1]), ax, ay);
+          const float s1 = sum + (ax + ay);
+          if (s1 <= 1.0995e12f) {
+            sum = s1;
+          } else {  // NaN too
+            const float2 r = careful_sum<T>(piece, Cfg::VPT, Cfg::Lanes, a.c2, ref, first ? 0.f : sum);
+            ref = r.x;
+            sum = r.y;
+            const float R = reference(ref, a.c2);
+            nR2 = f2(R, R);
+          }
+        } else if (left > 0) {  // the last piece, partly filled
+          const float2 r = careful_sum<T>(piece, min(left, Cfg::VPT), Cfg::Lanes, a.c2, ref, sum);
+          ref = r.x;
+          sum = r.y;
+        }
+        if (!a.grad) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.empty[slot]);
+        }
+        if (++slot == slots) {
+          slot = 0;
+          turn ^= 1;
+        }
+      }
+      if (!ok) break;
+      // Without a gradient nothing else makes a warp wait for the row before: a pair of row x
+      // may only leave once this block has all pairs of row x - 1.
+      if (!a.grad && x > 0 && !wait(&sh.pairs_full[(x - 1) & 1], (x - 1) >> 1)) break;
+      const float mw = warp_max(ref);
+      sum = warp_sum(Expo(a.c2, mw).join(ref, sum));
+      if (C == 1) {
+        if (lane == 0) {
+          sh.pairs[x & 1][warp] = make_float2(mw, sum);
+          mbar_arrive(&sh.pairs_full[x & 1]);
+        }
+      } else if (lane < C) {
+        const uint32_t to = mapa_shared(smem_u32(&sh.pairs[x & 1][rank * CW + warp]), (uint32_t)lane);
+        const uint32_t bar = mapa_shared(smem_u32(&sh.pairs_full[x & 1]), (uint32_t)lane);
+        st_async_f2(to, mw, sum, bar);
+      }
+      __syncwarp();
+      if (a.grad || warp == 0) {
+        if (!wait(&sh.pairs_full[x & 1], x >> 1)) break;
+        float m, tot;
+        join_pairs(sh.pairs[x & 1], C * CW, a.c2, lane, &m, &tot);
+        if (rank == 0 && warp == 0 && lane == 0) {
+          RowRecord* rec = reinterpret_cast<RowRecord*>(a.records) + t;
+          rec->m = m;
+          rec->sum = tot;
+        }
+        if (a.grad) {  // second pass
+        const Expo w(a.c2, m);
+        const float A = row_factor<OP>(a, token, w, tot, factor), As = A / tot;
+        if (OP == kOpDistill && warp == 0 && lane == 0) {
+          sh.factor[e][0] = A;
+          sh.factor[e][1] = As;
+          sh.factor[e][2] = m;
+        }
+        const F2 nM2 = f2(-w.M2, -w.M2), As2 = f2(As, As);
+        const bool plain = g.a == z.a && !w.far;
+        // whole vectors of this part: pieces within them take the straight path
+        const int lo = z.full(0) ? 0 : 1, hi = z.full(z.nv - 1) ? z.nv : z.nv - 1;
+        // the token's element belongs to the thread that writes its vector
+        const int own = OP == kOpDistill ? -1 : (int)(((int64_t)token.id + z.a) / N) - j0;
+        const bool own_mine = own >= 0 && own < j1 - j0 && own % Cfg::Lanes == tid;
+        const int own_piece = own_mine ? own / kPieceVecs : -1;
+        T* gp = g.p + z.first(j0 + tid);
+        int sl = slot0, left = mine;
+        for (int base = j0, n = 0; base < j1; base += kPieceVecs, ++n, left -= Cfg::VPT, gp += kPieceVecs * N) {
+          const uint4* piece = reinterpret_cast<const uint4*>(ring + (size_t)sl * kPieceBytes) + tid;
+          if (plain && base >= lo && base + kPieceVecs <= min(hi, j1)) {
+            uint4 raw[Cfg::VPT];
+#pragma unroll
+            for (int v = 0; v < Cfg::VPT; ++v) raw[v] = piece[v * Cfg::Lanes];
+#pragma unroll
+            for (int v = 0; v < Cfg::VPT; ++v) {
+              float o[N];
+              Elem<T>::unpack(raw[v], o);
+#pragma unroll
+              for (int i = 0; i < N; i += 2)
+                split(mul2(As2, ex2_2(fma2(f2(o[i], o[i + 1]), cc, nM2))), o[i], o[i + 1]);
+              *reinterpret_cast<uint4*>(gp + v * Cfg::Lanes * N) = Elem<T>::pack(o);
+            }
+          } else if (left > 0) {
+            careful_store<T>(piece, min(left, Cfg::VPT), Cfg::Lanes, g.p, a.V, z.first(base + tid), a.c2, m, As);
+          }
+          if (n == own_piece) g.p[token.id] = Elem<T>::t(As * w(token.z) - A);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.empty[sl]);
+          if (++sl == slots) sl = 0;
+        }
+        }
+      }
+      ++x;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(OP == kOpDistill ? &sh.dense_done[e] : &sh.ent_done[e]);
+      next_entry(e, lap);
+    }
+  }
+  if (*abort) {  // copies in flight land long before this
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 1000000) {
+    }
+  }
+  __syncthreads();
+  if (C > 1) cluster_sync();  // no block leaves while another may still write to it
+  if (*abort && threadIdx.x == 0) {
+    RowRecord* recs = reinterpret_cast<RowRecord*>(a.records);
+    for (int t = cluster; t < a.T; t += clusters) recs[t].state = kRowBad;
+  }
+}
+
+// Outputs of all rows from their records, one thread per row, and the loss as the sum over
+// rows in 64 bits: blocks leave partial sums, the last one adds them in their order, so the
+// loss has the same bits on every run. Log-probabilities are formed in 64 bits: in fp32 the
+// rounding of ln(sum) near 12 alone is 5e-7, and a sequence's log-ratio sums hundreds.
+constexpr int kFinishThreads = 256;
+template <int OP>
+__global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const VocabLossArgs a) {
+  __shared__ double red[32];
+  __shared__ bool last;
+  const int t = blockIdx.x * kFinishThreads + threadIdx.x;
+  const float nan = __int_as_float(0x7fffffff);
+  const double ln2 = 0.69314718055994530942;
+  float loss = 0.f;
+  if (t < a.T) {
+    const RowRecord r = reinterpret_cast<const RowRecord*>(a.records)[t];
+    const Expo x(a.c2, r.m);
+    double lp = 0.0;  // ln q of the token (of the entry that zref is from)
+    if (r.state == kRowOn)
+      lp = (x.far ? ((double)r.z - (double)r.m) * (double)a.c2 : (double)r.z * (double)a.c2 - (double)x.M2) * ln2 -
+           log((double)r.sum);
+    if constexpr (OP == kOpDistill) {
+      if (r.state == kRowOn) loss = (float)((double)a.tau * a.tau * (r.base - (double)r.weight * lp));
+      else if (r.state == kRowBad) loss = nan;
+    } else {
+      const bool on = r.state != kRowOff;
+      if (r.state == kRowBad) lp = (double)nan;
+      a.logp[t] = (float)lp;
+      if constexpr (OP == kOpLogp) {
+        if (a.lse) reinterpret_cast<float2*>(a.lse)[t] = on ? make_float2(r.m, r.sum) : make_float2(0.f, 0.f);
+        if (a.ratio) a.ratio[t] = on ? (float)(lp - (double)a.ref_logp[t]) : 0.f;
+      } else {
+        PolicyTerm o = {0.f, 0.f, 0.f};
+        if (on)
+          o = policy_term(a, a.adv[t], expf((float)(lp - (double)a.old_logp[t])),
+                          a.ref_logp ? (float)((double)a.ref_logp[t] - lp) : 0.f, a.ref_logp != nullptr);
+        loss = o.loss;
+        a.kl[t] = o.kl;
+      }
+    }
+  }
+  if constexpr (OP != kOpLogp) {
+    const double v = block_sum_d((double)loss, red);
+    if (threadIdx.x == 0) {
+      a.partial[blockIdx.x] = v;
+      __threadfence();
+      last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (last) {
+      __threadfence();
+      double s = 0.0;
+      for (int b = threadIdx.x; b < (int)gridDim.x; b += kFinishThreads) s += __ldcg(a.partial + b);
+      s = block_sum_d(s, red);
+      if (threadIdx.x == 0) *a.loss = (float)(a.count ? s / max(*a.count, 1) : s * (double)a.host_scale);
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------
@@ -390,30 +1015,6 @@ __global__ void __launch_bounds__(256) count_teacher_kernel(const void* ids, boo
   if (lane == 0 && n) atomicAdd(count, n);
 }
 
-__device__ __forceinline__ double block_sum_d(double v, double* s) {  // s: 32 doubles
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-  __syncthreads();
-  const int nw = blockDim.x >> 5;
-  v = (int)(threadIdx.x & 31) < nw ? s[threadIdx.x & 31] : 0.0;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-// One block: the same order of additions on every run, in 64 bits (a long sum of terms of
-// both signs).
-__global__ void __launch_bounds__(1024) rows_sum_kernel(const float* __restrict__ x, int n, float host_scale,
-                                                        const int* count, float* out) {
-  __shared__ double red[32];
-  double v = 0.0;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) v += x[i];
-  v = block_sum_d(v, red);
-  if (threadIdx.x == 0) *out = (float)(count ? v / max(*count, 1) : v * host_scale);
-}
-
 // The gradient is already in its type: one more rounding where the loss's own gradient is
 // not 1 (exact for powers of two).
 template <typename T>
@@ -435,7 +1036,7 @@ __global__ void __launch_bounds__(256) scale_grad_kernel(T* g, int64_t n, const 
 // ------------------------------------------------------------------------------------
 // Preference pairs: sequence 2 i is the chosen, 2 i + 1 the rejected one of pair i.
 // ------------------------------------------------------------------------------------
-// One block per pair. Log-ratios are summed in 64 bits: the margin is the difference of
+// One block per pair. Log-ratios, each rounded once from 64 bits, are summed in 64 bits: the margin is the difference of
 // two sums over whole sequences.
 __global__ void __launch_bounds__(256) preference_pairs_kernel(const PreferenceArgs a) {
   __shared__ double red[32];
@@ -447,7 +1048,7 @@ __global__ void __launch_bounds__(256) preference_pairs_kernel(const PreferenceA
     hi[s] = min(max(a.offsets[2 * i + s + 1], 0), a.T);
     double v = 0.0;
     for (int t = lo[s] + threadIdx.x; t < hi[s]; t += blockDim.x)
-      if (load_id(a.labels, t, a.ids64) >= 0) v += (double)a.logp[t] - (double)a.ref_logp[t];
+      v += (double)a.ratio[t];  // 0 where there is no label
     R[s] = (double)a.beta * block_sum_d(v, red);
   }
   const double m = R[0] - R[1], e = exp(-fabs(m));
@@ -467,6 +1068,15 @@ __global__ void __launch_bounds__(256) preference_pairs_kernel(const PreferenceA
   }
 }
 
+// One block: the mean over pairs, in a fixed order.
+__global__ void __launch_bounds__(256) preference_mean_kernel(const float* __restrict__ x, int n, float* out) {
+  __shared__ double red[32];
+  double v = 0.0;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) v += x[i];
+  v = block_sum_d(v, red);
+  if (threadIdx.x == 0) *out = (float)(v / max(n, 1));
+}
+
 // dz = up * row_coef * (onehot - softmax) from the saved log-sum-exp: one read, one write.
 template <typename T>
 __global__ void __launch_bounds__(256) preference_grad_kernel(const VocabLossArgs a, const float* __restrict__ row_coef,
@@ -481,14 +1091,16 @@ __global__ void __launch_bounds__(256) preference_grad_kernel(const VocabLossArg
   // rows outside the loss are not read: their logits may hold anything
   const bool on = label >= 0 && t >= a.offsets[0] && t < a.offsets[a.num_seq];
   const float A = on ? -coef * *a.up : 0.f;
-  const float2 l = reinterpret_cast<const float2*>(a.lse)[t];
+  const float2 l = reinterpret_cast<const float2*>(a.lse)[t];  // the row's maximum and sum
+  const Expo x(a.c2, l.x);
+  const float As = A / l.y;
   for (int j = j0 + threadIdx.x; j < j1; j += blockDim.x) {
     float o[N];
     if (on) {
       Elem<T>::unpack(z.load(j), o);
       const int64_t e0 = z.first(j);
 #pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = A * (ex2(fmaf(o[i] - l.x, a.c2, -l.y)) - (e0 + i == label ? 1.f : 0.f));
+      for (int i = 0; i < N; ++i) o[i] = fmaf(As, x(o[i]), e0 + i == label ? -A : 0.f);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) o[i] = 0.f;
@@ -497,13 +1109,119 @@ __global__ void __launch_bounds__(256) preference_grad_kernel(const VocabLossArg
   }
 }
 
-template <typename T>
-void launch_rows(const VocabLossArgs& a, int op, cudaStream_t st) {
-  const size_t sm = entries_bytes(op, a.K);
-  if (op == kOpDistill) vocab_row_kernel<T, kOpDistill><<<a.T, 512, sm, st>>>(a);
-  else if (op == kOpPolicy) vocab_row_kernel<T, kOpPolicy><<<a.T, 512, sm, st>>>(a);
-  else vocab_row_kernel<T, kOpLogp><<<a.T, 512, sm, st>>>(a);
+// Dynamic shared memory of a block, beside its static part and the system's 1 KB.
+template <typename Cfg>
+constexpr int stream_smem() {
+  return (228 * 1024 / Cfg::B - 1024 - (int)sizeof(StreamShared) - 256) & ~127;
+}
+
+template <typename Cfg>
+void stream_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute* at, int blocks, int C, int smem, cudaStream_t st) {
+  cfg->gridDim = dim3((unsigned)blocks);
+  cfg->blockDim = dim3(Cfg::Threads);
+  cfg->dynamicSmemBytes = (size_t)smem;
+  cfg->stream = st;
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)C;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg->attrs = at;
+  cfg->numAttrs = 1;
+}
+
+// Clusters of C blocks that fit on the device at once, per kernel and device.
+template <typename T, int OP, typename Cfg>
+int resident_clusters(int C, int smem) {
+  static std::mutex mu;
+  static std::map<std::array<int, 3>, int> known;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const std::lock_guard<std::mutex> lock(mu);
+  int& n = known[{dev, C, smem}];
+  if (!n) {
+    auto kernel = vocab_stream_kernel<T, OP, Cfg>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, stream_smem<Cfg>());
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    stream_config<Cfg>(&cfg, at, C, C, smem, nullptr);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+    if (e != cudaSuccess || n < 1) {
+      n = 0;
+      throw std::runtime_error(std::string("vocab_loss: ") + (e != cudaSuccess ? cudaGetErrorString(e) : "no room for a cluster"));
+    }
+  }
+  return n;
+}
+
+template <typename Cfg>
+int stream_slots(int ent) { return std::min(kMaxSlots, (stream_smem<Cfg>() - ent) / Cfg::PieceBytes); }
+template <typename Cfg>
+int stream_pieces(int nv, int C) { return ((nv + C - 1) / C + Cfg::PieceVecs - 1) / Cfg::PieceVecs; }
+
+template <typename T, int OP, typename Cfg>
+void launch_stream(const VocabLossArgs& a, int C, int rows_ahead, int ent, cudaStream_t st) {
+  const int slots = stream_slots<Cfg>(ent);
+  const int smem = slots * Cfg::PieceBytes + ent;
+  const int clusters = std::min(a.T, resident_clusters<T, OP, Cfg>(C, smem));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  stream_config<Cfg>(&cfg, at, clusters * C, C, smem, st);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, vocab_stream_kernel<T, OP, Cfg>, a, C, slots, rows_ahead);
+  if (e != cudaSuccess) throw std::runtime_error(std::string("vocab_loss: ") + cudaGetErrorString(e));
   check_launch("vocab_loss");
+}
+
+// One block of 16 warps per SM, or more and smaller blocks. What a row costs beside its
+// vectors (waits, the exchange of sums: some 3000 cycles) overlaps between the blocks of an
+// SM, so short rows want many small blocks and long ones the whole ring.
+using CfgBig = StreamCfg<16, 2, 1>;
+using CfgMid = StreamCfg<8, 2, 2>;
+using CfgSmall = StreamCfg<4, 2, 4>;
+using CfgTiny = StreamCfg<2, 2, 8>;
+
+// Whether rows of nv vectors take Cfg: one block holds a row and a part of the next one, and
+// there are more rows than blocks of the next larger kind.
+template <typename Cfg>
+bool stream_fits(int nv, int T, int ent, int num_sms) {
+  const int slots = stream_slots<Cfg>(ent);
+  return (int64_t)T > (int64_t)num_sms * (Cfg::B / 2) && stream_pieces<Cfg>(nv, 1) <= slots - slots / 4;
+}
+
+template <typename T, int OP>
+void launch_op(const VocabLossArgs& a, int num_sms, cudaStream_t st) {
+  constexpr int N = Elem<T>::N;
+  const int nv = (int)(((int64_t)a.V + 2 * N - 2) / N);  // vectors of a row at its worst phase
+  // distillation: entries of 4 rows, of 2 where they would take the ring's room
+  const int rows_ahead = OP != kOpDistill ? kTokens : a.K <= 256 ? 4 : 2;
+  const int ent = OP == kOpDistill ? rows_ahead * entries_padded(a.K) * kEntryBytes : 0;
+  if (stream_fits<CfgTiny>(nv, a.T, ent, num_sms)) return launch_stream<T, OP, CfgTiny>(a, 1, rows_ahead, ent, st);
+  if (stream_fits<CfgSmall>(nv, a.T, ent, num_sms)) return launch_stream<T, OP, CfgSmall>(a, 1, rows_ahead, ent, st);
+  if (stream_fits<CfgMid>(nv, a.T, ent, num_sms)) return launch_stream<T, OP, CfgMid>(a, 1, rows_ahead, ent, st);
+  // Blocks per row: as many as it takes for the row to stay in shared memory, and more
+  // while that leaves SMs without a row.
+  int C = 1;
+  const int slots = stream_slots<CfgBig>(ent);
+  while (C < kMaxCluster && (stream_pieces<CfgBig>(nv, C) > slots ||
+                             (stream_pieces<CfgBig>(nv, C) > 1 && (int64_t)a.T * C * 2 <= num_sms)))
+    C *= 2;
+  if (stream_pieces<CfgBig>(nv, C) <= slots) return launch_stream<T, OP, CfgBig>(a, C, rows_ahead, ent, st);
+  vocab_row_kernel<T, OP><<<a.T, 512, OP == kOpDistill ? entries_padded(a.K) * kEntryBytes : 16, st>>>(a);
+  check_launch("vocab_loss");
+}
+
+template <typename T>
+void launch_rows(const VocabLossArgs& a, int op, int num_sms, cudaStream_t st) {
+  const int blocks = vocab_finish_blocks(a.T);
+  if (op == kOpDistill) {
+    launch_op<T, kOpDistill>(a, num_sms, st);
+    vocab_finish_kernel<kOpDistill><<<blocks, kFinishThreads, 0, st>>>(a);
+  } else if (op == kOpPolicy) {
+    launch_op<T, kOpPolicy>(a, num_sms, st);
+    vocab_finish_kernel<kOpPolicy><<<blocks, kFinishThreads, 0, st>>>(a);
+  } else {
+    launch_op<T, kOpLogp>(a, num_sms, st);
+    vocab_finish_kernel<kOpLogp><<<blocks, kFinishThreads, 0, st>>>(a);
+  }
+  check_launch("vocab_finish");
 }
 
 }  // namespace
@@ -517,18 +1235,18 @@ void vocab_count_rows(const VocabLossArgs& a, int op, int* count, cudaStream_t s
   check_launch("vocab_count_rows");
 }
 
-void vocab_loss(const VocabLossArgs& a, int op, cudaStream_t st) {
-  if (a.T <= 0) return;
+int vocab_finish_blocks(int T) { return (T + kFinishThreads - 1) / kFinishThreads; }
+
+void vocab_loss(const VocabLossArgs& a, int op, int num_sms, cudaStream_t st) {
+  if (a.T <= 0) {  // a loss over nothing
+    if (a.loss) cudaMemsetAsync(a.loss, 0, sizeof(float), st);
+    return;
+  }
   if (a.V < 1) throw std::runtime_error("vocab_loss: empty vocabulary");
   if (op == kOpDistill && (a.K < 1 || a.K > kMaxTeacher)) throw std::runtime_error("vocab_loss: teacher entries");
-  if (a.dtype == kVocabBf16) launch_rows<__nv_bfloat16>(a, op, st);
-  else if (a.dtype == kVocabF16) launch_rows<__half>(a, op, st);
-  else launch_rows<float>(a, op, st);
-}
-
-void vocab_loss_sum(const VocabLossArgs& a, float* loss, cudaStream_t st) {
-  rows_sum_kernel<<<1, 1024, 0, st>>>(a.row_loss, a.T, a.host_scale, a.count, loss);
-  check_launch("vocab_loss_sum");
+  if (a.dtype == kVocabBf16) launch_rows<__nv_bfloat16>(a, op, num_sms, st);
+  else if (a.dtype == kVocabF16) launch_rows<__half>(a, op, num_sms, st);
+  else launch_rows<float>(a, op, num_sms, st);
 }
 
 void vocab_scale_grad(void* grad, int dtype, int64_t n, const float* up, int num_sms, cudaStream_t st) {
@@ -547,7 +1265,7 @@ void preference_pairs(const PreferenceArgs& a, cudaStream_t st) {
 }
 
 void preference_loss_sum(const float* pair_loss, int pairs, float* loss, cudaStream_t st) {
-  rows_sum_kernel<<<1, 1024, 0, st>>>(pair_loss, pairs, 1.f / (float)std::max(pairs, 1), nullptr, loss);
+  preference_mean_kernel<<<1, 256, 0, st>>>(pair_loss, pairs, loss);
   check_launch("preference_loss_sum");
 }
 

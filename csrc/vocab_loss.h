@@ -23,7 +23,8 @@ struct VocabLossArgs {
   int dtype = kVocabBf16;
   int T = 0, V = 0;
   float c2 = 0.f;            // log2(e) / temperature
-  float tau = 1.f;           // temperature
+  float tau = 1.f;           // temperature, and unrounded
+  double tau64 = 1.0;
   float host_scale = 1.f;    // 1 / rows in the loss, when the host knows it ...
   const int* count = nullptr;  // ... else the number of rows, on the device
   const float* up = nullptr;   // optional gradient of the loss, on the device
@@ -40,25 +41,29 @@ struct VocabLossArgs {
   float clip_low = 0.f, clip_high = 0.f, kl_coef = 0.f;
   const int* offsets = nullptr;  // kOpLogp: rows outside [offsets[0], offsets[num_seq]) are not in the loss
   int num_seq = 0;
-  // outputs, [T] fp32
-  float* row_loss = nullptr;  // kOpDistill / kOpPolicy
-  float* logp = nullptr;      // kOpPolicy / kOpLogp
-  float* kl = nullptr;        // kOpPolicy
-  float* lse = nullptr;       // kOpLogp: [T, 2], the row's maximum and log2 of sum 2^((z - max) c2)
+  // scratch
+  void* records = nullptr;     // [T] records of kRowRecordBytes each
+  double* partial = nullptr;   // [vocab_finish_blocks(T)]
+  unsigned int* ticket = nullptr;  // [1], needs no value
+  // outputs, fp32
+  float* loss = nullptr;  // [1], kOpDistill / kOpPolicy: the mean over rows
+  float* logp = nullptr;  // [T], kOpPolicy / kOpLogp
+  float* kl = nullptr;    // [T], kOpPolicy
+  float* ratio = nullptr;  // [T], kOpLogp: logp - ref_logp, 0 for rows not in the loss (optional)
+  float* lse = nullptr;    // [T, 2], kOpLogp: a reference m of the row and its sum of 2^((z - m) c2) (optional)
 };
+constexpr int kRowRecordBytes = 32;
+int vocab_finish_blocks(int T);
 
 // Rows in the loss: *count = number of rows with a label >= 0 (labels [T]), or with a
 // teacher entry (ids / teacher [T, K]). count must be zero before the call.
 void vocab_count_rows(const VocabLossArgs& a, int op, int* count, cudaStream_t st);
-void vocab_loss(const VocabLossArgs& a, int op, cudaStream_t st);
-// *loss = sum(row_loss[0..T)) / rows (host_scale or count), in a fixed order.
-void vocab_loss_sum(const VocabLossArgs& a, float* loss, cudaStream_t st);
+void vocab_loss(const VocabLossArgs& a, int op, int num_sms, cudaStream_t st);
 // grad *= *up, in place; nothing is touched where *up is 1.
 void vocab_scale_grad(void* grad, int dtype, int64_t n, const float* up, int num_sms, cudaStream_t st);
 
 struct PreferenceArgs {
-  const float* logp = nullptr;   // [T]
-  const float* ref_logp = nullptr;  // [T]
+  const float* ratio = nullptr;  // [T] logp - ref_logp, 0 for rows not in the loss
   const void* labels = nullptr;  // [T]
   bool ids64 = false;
   const int* offsets = nullptr;  // [2 * pairs + 1]

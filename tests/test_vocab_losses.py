@@ -137,7 +137,8 @@ def _distill_inputs(T, V, K, dtype, strided, seed=0):
     return z, ids.cuda(), t.cuda()
 
 
-CASES = [(1, 1, 1), (1, 7, 3), (3, 8, 8), (5, 257, 2), (4, 4104, 64), (3, 50257, 300), (2, 151936, 16)]
+CASES = [(1, 1, 1), (1, 7, 3), (3, 8, 8), (5, 257, 2), (4, 4104, 64), (3, 50257, 300), (2, 151936, 16),
+         (500, 300, 5), (330, 20011, 40), (2, 900001, 12)]
 
 
 @pytest.mark.gpu
@@ -179,7 +180,8 @@ def _policy_inputs(T, V, dtype, strided, seed=0, tau=1.0):
 @pytest.mark.gpu
 @pytest.mark.parametrize("strided", [False, True])
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
-@pytest.mark.parametrize("T,V", [(1, 1), (1, 9), (4, 8), (67, 257), (9, 4104), (5, 50257), (3, 151936)])
+@pytest.mark.parametrize("T,V", [(1, 1), (1, 9), (4, 8), (67, 257), (9, 4104), (5, 50257), (3, 151936), (700, 301), (331, 20011),
+                                 (2, 900001)])
 def test_policy(T, V, dtype, strided):
     from spec_ep.ops.loss import clipped_policy_loss
 
@@ -211,7 +213,8 @@ def test_preference_reference_margin_sign():
 @pytest.mark.parametrize("strided", [False, True])
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("off,tail,V", [([0, 1, 2], 0, 9), ([0, 3, 3, 10, 11], 0, 257), ([2, 9, 300, 301, 340], 6, 520),
-                                        ([0, 5, 12], 1, 50257), ([0, 2, 3], 0, 151936)])
+                                        ([0, 5, 12], 1, 50257), ([0, 2, 3], 0, 151936), ([1, 50, 333, 400, 640], 9, 5003),
+                                        ([0, 1, 2], 0, 900001)])
 def test_preference(off, tail, V, dtype, strided):
     from spec_ep.ops.loss import preference_loss, token_logp
 
