@@ -2,6 +2,7 @@
 // loss (router_balance.cu).
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -350,15 +351,181 @@ at::Tensor router_balance_bwd(const at::Tensor& x, const at::Tensor& topk_e, con
   return dx;
 }
 
+// ------------------------------------------------------------------------------------
+// Autograd. The nodes are C++ ones: a Python node would take the interpreter lock on the
+// engine's thread, which costs as much as a small batch's kernels.
+// ------------------------------------------------------------------------------------
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool wants_grad(const at::Tensor& z) { return at::GradMode::is_enabled() && z.requires_grad(); }
+
+// Gradients here are not themselves differentiable: whoever tries, through the logits that
+// they depend on, gets an error.
+at::Tensor once(AutogradContext* ctx, const at::Tensor& g) {
+  if (!at::GradMode::is_enabled()) return g;
+  auto error = std::make_shared<torch::autograd::DelayedError>("this loss can only be differentiated once", 2);
+  return (*error)({g, ctx->get_saved_variables()[0]})[0];
+}
+
+// A loss whose forward has formed the gradient in its pass over the logits. It is handed out
+// once, scaled in place (not touched where the upstream gradient is 1). A second backward
+// through the same graph, and fp16 logits, whose unscaled gradient could leave the type's
+// range, compute it from the logits.
+at::Tensor gradient_buffer(const at::Tensor& z) { return at::empty(z.sizes(), z.options()); }
+bool formed_in_forward(const at::Tensor& z) { return z.scalar_type() != at::kHalf; }
+at::Tensor take_formed(AutogradContext* ctx, const at::Tensor& up) {
+  auto& kept = ctx->saved_data["grad"];
+  if (!kept.isTensor()) return {};
+  at::Tensor g = kept.toTensor();
+  kept = c10::IValue();
+  scale_grad(g, up);
+  return g;
+}
+
+struct DistillFn : torch::autograd::Function<DistillFn> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& z, const at::Tensor& ids, const at::Tensor& teacher,
+                            double tau, int64_t num_valid) {
+    c10::optional<at::Tensor> grad;
+    if (formed_in_forward(z)) ctx->saved_data["grad"] = *(grad = gradient_buffer(z));
+    at::Tensor loss = distill_loss(z, ids, teacher, tau, num_valid, grad, c10::nullopt);
+    ctx->save_for_backward({z, ids, teacher});
+    ctx->saved_data["tau"] = tau;
+    ctx->saved_data["num_valid"] = num_valid;
+    return loss;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list up) {
+    at::Tensor g = take_formed(ctx, up[0]);
+    if (!g.defined()) {
+      const auto s = ctx->get_saved_variables();
+      g = gradient_buffer(s[0]);
+      distill_loss(s[0], s[1], s[2], ctx->saved_data["tau"].toDouble(), ctx->saved_data["num_valid"].toInt(), g, up[0]);
+    }
+    return {once(ctx, g), {}, {}, {}, {}};
+  }
+};
+
+at::Tensor topk_distill(const at::Tensor& z, const at::Tensor& ids, const at::Tensor& teacher, double tau,
+                        int64_t num_valid) {
+  if (!wants_grad(z)) return distill_loss(z, ids, teacher, tau, num_valid, c10::nullopt, c10::nullopt);
+  return DistillFn::apply(z, ids, teacher, tau, num_valid);
+}
+
+struct PolicyFn : torch::autograd::Function<PolicyFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& z, const at::Tensor& actions,
+                               const at::Tensor& old_logp, const at::Tensor& advantages,
+                               const c10::optional<at::Tensor>& ref_logp, double clip_low, double clip_high,
+                               double kl_coef, double tau, int64_t num_valid) {
+    c10::optional<at::Tensor> grad;
+    if (formed_in_forward(z)) ctx->saved_data["grad"] = *(grad = gradient_buffer(z));
+    auto out = policy_loss(z, actions, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coef, tau, num_valid,
+                           grad, c10::nullopt);
+    ctx->save_for_backward({z, actions, old_logp, advantages, ref_logp.value_or(at::Tensor())});
+    ctx->saved_data["cfg"] = std::vector<double>{clip_low, clip_high, kl_coef, tau};
+    ctx->saved_data["num_valid"] = num_valid;
+    ctx->mark_non_differentiable({out[1], out[2]});
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list up) {
+    at::Tensor g;
+    if (up[0].defined()) {
+      g = take_formed(ctx, up[0]);
+      if (!g.defined()) {
+        const auto s = ctx->get_saved_variables();
+        const auto c = ctx->saved_data["cfg"].toDoubleVector();
+        g = gradient_buffer(s[0]);
+        policy_loss(s[0], s[1], s[2], s[3], s[4].defined() ? c10::optional<at::Tensor>(s[4]) : c10::nullopt, c[0], c[1],
+                    c[2], c[3], ctx->saved_data["num_valid"].toInt(), g, up[0]);
+      }
+      g = once(ctx, g);
+    }
+    return {g, {}, {}, {}, {}, {}, {}, {}, {}, {}};
+  }
+};
+
+std::vector<at::Tensor> clipped_policy(const at::Tensor& z, const at::Tensor& actions, const at::Tensor& old_logp,
+                                       const at::Tensor& advantages, const c10::optional<at::Tensor>& ref_logp,
+                                       double clip_low, double clip_high, double kl_coef, double tau,
+                                       int64_t num_valid) {
+  if (!wants_grad(z))
+    return policy_loss(z, actions, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coef, tau, num_valid,
+                       c10::nullopt, c10::nullopt);
+  return PolicyFn::apply(z, actions, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coef, tau, num_valid);
+}
+
+struct PreferenceFn : torch::autograd::Function<PreferenceFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& z, const at::Tensor& labels,
+                               const at::Tensor& offsets, const at::Tensor& ref_logp, double beta, double eps) {
+    auto out = preference_fwd(z, labels, offsets, ref_logp, beta, eps, c10::nullopt);
+    ctx->save_for_backward({z, labels, offsets, out[3], out[4]});
+    out.resize(3);
+    ctx->mark_non_differentiable({out[1], out[2]});
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list up) {
+    at::Tensor g;
+    if (up[0].defined()) {
+      const auto s = ctx->get_saved_variables();
+      g = once(ctx, preference_grad(s[0], s[1], s[2], s[3], s[4], up[0]));
+    }
+    return {g, {}, {}, {}, {}, {}};
+  }
+};
+
+// Returns (loss, rewards, logp).
+std::vector<at::Tensor> preference(const at::Tensor& z, const at::Tensor& labels, const at::Tensor& offsets,
+                                   const at::Tensor& ref_logp, double beta, double eps) {
+  if (wants_grad(z)) return PreferenceFn::apply(z, labels, offsets, ref_logp, beta, eps);
+  auto out = preference_fwd(z, labels, offsets, ref_logp, beta, eps, c10::nullopt);
+  out.resize(3);
+  return out;
+}
+
+struct RouterBalanceFn : torch::autograd::Function<RouterBalanceFn> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, int64_t k, bool renorm,
+                               const c10::optional<at::Tensor>& bias, const c10::optional<at::Tensor>& valid) {
+    auto out = router_balance_fwd(x, k, renorm, bias, valid);
+    ctx->save_for_backward({x, out[1], out[4], valid.value_or(at::Tensor())});
+    ctx->saved_data["renorm"] = renorm;
+    out.resize(4);
+    ctx->mark_non_differentiable({out[1], out[3]});
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list up) {
+    at::Tensor g;
+    if (up[0].defined() || up[2].defined()) {
+      const auto s = ctx->get_saved_variables();
+      auto opt = [](const at::Tensor& t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; };
+      g = once(ctx, router_balance_bwd(s[0], s[1], s[2], ctx->saved_data["renorm"].toBool(), opt(s[3]),
+                                  opt(up[0].defined() ? up[0].contiguous() : up[0]), opt(up[2])));
+    }
+    return {g, {}, {}, {}, {}};
+  }
+};
+
+// Returns (topk_w, topk_e, loss, counts).
+std::vector<at::Tensor> router_balanced(const at::Tensor& x, int64_t k, bool renorm,
+                                        const c10::optional<at::Tensor>& bias,
+                                        const c10::optional<at::Tensor>& valid) {
+  if (wants_grad(x)) return RouterBalanceFn::apply(x, k, renorm, bias, valid);
+  auto out = router_balance_fwd(x, k, renorm, bias, valid);
+  out.resize(4);
+  return out;
+}
+
 }  // namespace
 
 void register_losses(pybind11::module& m) {
+  m.def("topk_distill", &topk_distill);
+  m.def("clipped_policy", &clipped_policy);
+  m.def("preference", &preference);
+  m.def("router_balanced", &router_balanced);
+  m.def("token_logp", &token_logp);
+  // without autograd; the gradient may overwrite the logits
   m.def("distill_loss", &distill_loss);
   m.def("policy_loss", &policy_loss);
-  m.def("token_logp", &token_logp);
   m.def("preference_fwd", &preference_fwd);
-  m.def("preference_grad", &preference_grad);
-  m.def("scale_grad", &scale_grad);
-  m.def("router_balance_fwd", &router_balance_fwd);
-  m.def("router_balance_bwd", &router_balance_bwd);
 }

@@ -19,7 +19,6 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ._ext import load
 from .linear import dense_dgrad, dense_fwd, dense_wgrad
@@ -79,44 +78,9 @@ def _valid(num_valid):
     return int(num_valid)
 
 
-def _wants_grad(logits):
-    return torch.is_grad_enabled() and logits.requires_grad
-
-
-def _hand_over(ctx, up, again):
-    """Gradient of the logits for upstream ``up``. The forward formed it in its pass over
-    the logits; it is handed out once, scaled in place (not touched where ``up`` is 1). A
-    second backward through the same graph, or fp16 logits, whose unscaled gradient could
-    leave the type's range, compute it from the logits."""
-    grad, ctx.grad = ctx.grad, None
-    up = up.contiguous()
-    if grad is None:
-        return again(up)
-    load().scale_grad(grad, up)
-    return grad
-
-
-class _TopkDistill(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, ids, teacher, tau, num_valid, want):
-        ctx.grad = logits.new_empty(logits.shape) if want and logits.dtype != torch.float16 else None
-        loss = load().distill_loss(logits, ids, teacher, tau, num_valid, ctx.grad, None)
-        ctx.save_for_backward(logits, ids, teacher)
-        ctx.cfg = (tau, num_valid)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, up):
-        logits, ids, teacher = ctx.saved_tensors
-        tau, num_valid = ctx.cfg
-
-        def again(up):
-            grad = logits.new_empty(logits.shape)
-            load().distill_loss(logits, ids, teacher, tau, num_valid, grad, up)
-            return grad
-
-        return _hand_over(ctx, up, again), None, None, None, None, None
+def _f32(t):
+    """An input that gets no gradient, in fp32."""
+    return t.detach().float().contiguous()
 
 
 def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
@@ -133,47 +97,14 @@ def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     ``num_valid`` (rows with an entry, if the host knows it) spares a count on the device.
     Gradients reach ``logits`` only.
     """
-    return _TopkDistill.apply(logits, teacher_ids.contiguous(), teacher_logits.detach().float().contiguous(),
-                              float(temperature), _valid(num_valid), _wants_grad(logits))
+    return load().topk_distill(logits, teacher_ids.contiguous(), _f32(teacher_logits), float(temperature),
+                               _valid(num_valid))
 
 
 class PolicyLoss(NamedTuple):
     loss: torch.Tensor  # scalar
     logp: torch.Tensor  # [T] log-probability of each action (0 where there is none)
     kl: torch.Tensor    # [T] estimate of the KL to the reference model (0 without one)
-
-
-class _ClippedPolicy(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, actions, old_logp, advantages, ref_logp, cfg, want):
-        ctx.grad = logits.new_empty(logits.shape) if want and logits.dtype != torch.float16 else None
-        loss, logp, kl = load().policy_loss(logits, actions, old_logp, advantages, ref_logp, cfg[0], cfg[1], cfg[2],
-                                            cfg[3], cfg[4], ctx.grad, None)
-        ctx.save_for_backward(logits, actions, old_logp, advantages, ref_logp)
-        ctx.cfg = cfg
-        ctx.mark_non_differentiable(logp, kl)
-        ctx.set_materialize_grads(False)
-        return loss, logp, kl
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, up, _dlogp, _dkl):
-        if up is None:
-            return None, None, None, None, None, None, None
-        logits, actions, old_logp, advantages, ref_logp = ctx.saved_tensors
-        cfg = ctx.cfg
-
-        def again(up):
-            grad = logits.new_empty(logits.shape)
-            load().policy_loss(logits, actions, old_logp, advantages, ref_logp, cfg[0], cfg[1], cfg[2], cfg[3],
-                               cfg[4], grad, up)
-            return grad
-
-        return _hand_over(ctx, up, again), None, None, None, None, None, None
-
-
-def _f32_rows(t):
-    return None if t is None else t.detach().float().contiguous()
 
 
 def clipped_policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logp: torch.Tensor,
@@ -194,9 +125,10 @@ def clipped_policy_loss(logits: torch.Tensor, actions: torch.Tensor, old_logp: t
     the vocabulary makes the loss NaN. ``num_valid`` (rows with an action, if the host
     knows it) spares a count on the device. Gradients reach ``logits`` only.
     """
-    cfg = (float(clip_low), float(clip_high), float(kl_coef), float(temperature), _valid(num_valid))
-    return PolicyLoss(*_ClippedPolicy.apply(logits, actions.contiguous(), _f32_rows(old_logp), _f32_rows(advantages),
-                                            _f32_rows(ref_logp), cfg, _wants_grad(logits)))
+    return PolicyLoss(*load().clipped_policy(logits, actions.contiguous(), _f32(old_logp), _f32(advantages),
+                                             None if ref_logp is None else _f32(ref_logp), float(clip_low),
+                                             float(clip_high), float(kl_coef), float(temperature),
+                                             _valid(num_valid)))
 
 
 def token_logp(logits: torch.Tensor, labels: torch.Tensor, temperature: float = 1.0) -> torch.Tensor:
@@ -210,25 +142,6 @@ class PreferenceLoss(NamedTuple):
     loss: torch.Tensor     # scalar
     rewards: torch.Tensor  # [2 * pairs] beta * (sum of logp - ref_logp) of each sequence
     logp: torch.Tensor     # [T] log-probability of each label (0 where there is none)
-
-
-class _Preference(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, offsets, ref_logp, beta, eps):
-        loss, rewards, logp, lse, coef = load().preference_fwd(logits, labels, offsets, ref_logp, beta, eps, None)
-        ctx.save_for_backward(logits, labels, offsets, lse, coef)
-        ctx.mark_non_differentiable(rewards, logp)
-        ctx.set_materialize_grads(False)
-        return loss, rewards, logp
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, up, _drewards, _dlogp):
-        if up is None:
-            return None, None, None, None, None, None
-        logits, labels, offsets, lse, coef = ctx.saved_tensors
-        grad = load().preference_grad(logits, labels, offsets, lse, coef, up.contiguous())
-        return grad, None, None, None, None, None
 
 
 def preference_loss(logits: torch.Tensor, labels: torch.Tensor, seq_offsets: torch.Tensor, ref_logp: torch.Tensor,
@@ -247,5 +160,5 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, seq_offsets: tor
     read and their gradient is 0. A label outside the vocabulary makes the loss NaN.
     Gradients reach ``logits`` only.
     """
-    return PreferenceLoss(*_Preference.apply(logits, labels.contiguous(), seq_offsets.contiguous(),
-                                             _f32_rows(ref_logp), float(beta), float(label_smoothing)))
+    return PreferenceLoss(*load().preference(logits, labels.contiguous(), seq_offsets.contiguous(), _f32(ref_logp),
+                                             float(beta), float(label_smoothing)))

@@ -51,26 +51,6 @@ def router_topk_reference(logits, k, renorm=True, bias=None):
     return w, idx.int()
 
 
-class _RouterTopKBalanced(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, k, renorm, bias, valid):
-        w, e, loss, counts, coef = load().router_balance_fwd(logits, k, renorm, bias, valid)
-        ctx.save_for_backward(logits, e, coef, valid)
-        ctx.renorm = renorm
-        ctx.mark_non_differentiable(e, counts)
-        ctx.set_materialize_grads(False)
-        return w, e, loss, counts
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dw, _de, dloss, _dcounts):
-        if dw is None and dloss is None:
-            return None, None, None, None, None
-        logits, e, coef, valid = ctx.saved_tensors
-        dw = dw.contiguous() if dw is not None else None
-        return load().router_balance_bwd(logits, e, coef, ctx.renorm, valid, dw, dloss), None, None, None, None
-
-
 def router_topk_balanced(logits: torch.Tensor, k: int, renorm: bool = True, bias: torch.Tensor | None = None,
                          valid: torch.Tensor | None = None):
     """Top-k routing with a load-balance loss: ``(topk_w, topk_e, loss, counts)``.
@@ -87,7 +67,7 @@ def router_topk_balanced(logits: torch.Tensor, k: int, renorm: bool = True, bias
     they are routed all the same. With no token left the loss is 0. Among equal scores the
     lowest expert index is chosen; a NaN score is chosen before any number.
     """
-    return _RouterTopKBalanced.apply(logits, int(k), bool(renorm), bias, valid)
+    return tuple(load().router_balanced(logits, int(k), bool(renorm), bias, valid))
 
 
 def router_topk_balanced_reference(logits, k, renorm=True, bias=None, valid=None):

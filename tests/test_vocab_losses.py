@@ -532,3 +532,33 @@ def test_refusals():
     _refused(preference_loss, z, i, off, f[:3], match="ref_logp")
     _refused(preference_loss, z, i, off, f, beta=0.0, match="beta")
     _refused(preference_loss, z, i, off, f, label_smoothing=0.5, match="label_smoothing")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", [0, 1, 2])
+def test_backward_twice_needs_a_kept_graph_and_gradients_are_not_differentiable(i):
+    z, _ = _logits(33, 515, "bf16", False, 1)
+    loss = _three(z, i)
+    torch.autograd.grad(loss, z)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, z)
+    (g,) = torch.autograd.grad(_three(z, i), z, create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(g.float().sum(), z)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("i", [0, 1, 2])
+def test_gradient_reaches_a_leaf_behind_other_operations(i):
+    """z = w * x: the losses' gradient goes on through the product, twice into one .grad."""
+    x, _ = _logits(33, 515, "fp32", False, 1)
+    w = torch.full((515,), 1.5, device="cuda", requires_grad=True)
+    (g,) = torch.autograd.grad(_three((x.detach() * 1.5).requires_grad_(), i).sum() * 0 + _three(x * w, i), x)
+    z = (x.detach() * 1.5).requires_grad_()
+    (gz,) = torch.autograd.grad(_three(z, i), z)
+    assert torch.equal(g, gz * 1.5)
+    leaf = x.detach().clone().requires_grad_()
+    for _ in range(2):
+        _three(leaf, i).backward()
+    (once,) = torch.autograd.grad(_three(leaf, i), leaf)
+    assert torch.equal(leaf.grad, 2 * once)
