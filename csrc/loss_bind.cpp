@@ -1,6 +1,7 @@
 // Python bindings of the vocabulary losses (vocab_loss.cu) and of the router with a balance
 // loss (router_balance.cu).
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -85,7 +86,7 @@ at::Tensor set_rows(sepx::VocabLossArgs& a, int op, int64_t num_valid, const at:
   if (num_valid >= 0) {
     a.host_scale = 1.f / (float)std::max<int64_t>(num_valid, 1);
   } else {
-    count = at::zeros({1}, z.options().dtype(at::kInt));
+    count = a.T > 0 ? at::empty({1}, z.options().dtype(at::kInt)) : at::zeros({1}, z.options().dtype(at::kInt));
     a.count = count.data_ptr<int>();
     sepx::vocab_count_rows(a, op, count.data_ptr<int>(), cs());
   }
@@ -93,8 +94,9 @@ at::Tensor set_rows(sepx::VocabLossArgs& a, int op, int64_t num_valid, const at:
 }
 
 // Scratch of a call: records, partial sums and a ticket in one allocation.
-at::Tensor set_scratch(sepx::VocabLossArgs& a, const at::Tensor& z) {
-  const int64_t rec = (int64_t)a.T * sepx::kRowRecordBytes, part = (int64_t)sepx::vocab_finish_blocks(a.T) * 8;
+at::Tensor set_scratch(sepx::VocabLossArgs& a, const at::Tensor& z, int64_t partial = 0) {
+  const int64_t rec = (int64_t)a.T * sepx::kRowRecordBytes;
+  const int64_t part = std::max<int64_t>(sepx::vocab_finish_blocks(a.T), partial) * 8;
   at::Tensor s = at::empty({rec + part + 16}, z.options().dtype(at::kByte));
   uint8_t* p = s.data_ptr<uint8_t>();
   a.records = p;
@@ -188,8 +190,9 @@ void set_offsets(sepx::VocabLossArgs& a, const at::Tensor& offsets, const at::Te
   a.num_seq = (int)offsets.size(0) - 1;
 }
 
-// Returns (loss, rewards [2 * pairs], logp [T], lse [T, 2], row_coef [T] = d loss / d logp).
-// With `grad` (may be the logits), d logp / d logits of each row is written there, negated.
+// Returns (loss, rewards [2 * pairs], logp [T], rows [4, T]: the rows' lse as T pairs, then
+// d loss / d logp, then scratch). With `grad` (may be the logits), d logp / d logits of each
+// row is written there, negated.
 std::vector<at::Tensor> preference_fwd(const at::Tensor& z, const at::Tensor& labels, const at::Tensor& offsets,
                                        const at::Tensor& ref_logp, double beta, double eps,
                                        const c10::optional<at::Tensor>& grad) {
@@ -203,53 +206,52 @@ std::vector<at::Tensor> preference_fwd(const at::Tensor& z, const at::Tensor& la
   need_cuda(z, "logits");
   const c10::cuda::CUDAGuard guard(z.device());
   a.labels = labels.data_ptr();
-  const auto f32 = z.options().dtype(at::kFloat);
-  at::Tensor logp = at::empty({a.T}, f32), lse = at::empty({a.T, 2}, f32);
-  a.logp = logp.data_ptr<float>();
-  at::Tensor ratio = at::empty({a.T}, f32);
-  a.lse = lse.data_ptr<float>();
-  a.ref_logp = ref_logp.data_ptr<float>();
-  a.ratio = ratio.data_ptr<float>();
-  const at::Tensor scratch = set_scratch(a, z);
-  sepx::vocab_loss(a, sepx::kOpLogp, sms(), cs());
-
   sepx::PreferenceArgs q;
+  q.pairs = a.num_seq / 2;
+  const auto f32 = z.options().dtype(at::kFloat);
+  at::Tensor loss = at::empty({}, f32), rewards = at::empty({2 * (int64_t)q.pairs}, f32);
+  at::Tensor logp = at::empty({a.T}, f32), rows = at::empty({4, a.T}, f32);
+  const at::Tensor scratch = set_scratch(a, z, q.pairs);
+  a.logp = logp.data_ptr<float>();
+  a.lse = rows.data_ptr<float>();
+  a.row_coef = a.lse + 2 * (int64_t)a.T;
+  a.ratio = a.lse + 3 * (int64_t)a.T;
+  a.ref_logp = ref_logp.data_ptr<float>();
+  if (a.T > 0) sepx::vocab_loss(a, sepx::kOpLogp, sms(), cs());
+  else if (q.pairs > 0) C10_CUDA_CHECK(cudaMemsetAsync(a.ticket, 0, sizeof(int), cs()));
   q.ratio = a.ratio;
   q.labels = a.labels;
   q.ids64 = a.ids64;
   q.offsets = a.offsets;
   q.T = a.T;
-  q.pairs = a.num_seq / 2;
   q.beta = (float)beta;
   q.eps = (float)eps;
-  at::Tensor loss = at::empty({}, f32), rewards = at::empty({2 * (int64_t)q.pairs}, f32);
-  at::Tensor pair_loss = at::empty({q.pairs}, f32), row_coef = at::zeros({a.T}, f32);
   q.rewards = rewards.data_ptr<float>();
-  q.pair_loss = pair_loss.data_ptr<float>();
-  q.row_coef = row_coef.data_ptr<float>();
+  q.loss = loss.data_ptr<float>();
+  q.row_coef = a.row_coef;
+  q.partial = a.partial;
+  q.ticket = a.ticket;
   sepx::preference_pairs(q, cs());
-  sepx::preference_loss_sum(q.pair_loss, q.pairs, loss.data_ptr<float>(), cs());
-  return {loss, rewards, logp, lse, row_coef};
+  return {loss, rewards, logp, rows};
 }
 
-// d (up * loss) / d logits from the forward's lse and row_coef.
+// d (up * loss) / d logits from the forward's rows.
 at::Tensor preference_grad(const at::Tensor& z, const at::Tensor& labels, const at::Tensor& offsets,
-                           const at::Tensor& lse, const at::Tensor& row_coef, const at::Tensor& up) {
-  at::Tensor grad = at::empty(z.sizes(), z.options().memory_format(at::MemoryFormat::Contiguous));
+                           const at::Tensor& rows, const at::Tensor& up) {
+  at::Tensor grad = at::empty(z.sizes(), z.options());
   auto a = vocab_args(z, grad, 1.0);
   req_rows(labels, z, "labels");
-  req_f32_rows(row_coef, z, "row_coef");
-  TORCH_CHECK(lse.device() == z.device() && lse.scalar_type() == at::kFloat && lse.is_contiguous() &&
-                  lse.numel() == 2 * z.size(0),
-              "lse must be [T, 2] fp32");
+  TORCH_CHECK(rows.device() == z.device() && rows.scalar_type() == at::kFloat && rows.is_contiguous() &&
+                  rows.numel() == 4 * z.size(0),
+              "rows must be the forward's");
   set_offsets(a, offsets, z);
+  a.ids64 = ids_are_64(labels, "labels");
   need_cuda(z, "logits");
   const c10::cuda::CUDAGuard guard(z.device());
   a.labels = labels.data_ptr();
-  a.ids64 = ids_are_64(labels, "labels");
-  a.lse = lse.data_ptr<float>();
+  a.lse = rows.data_ptr<float>();
   set_upstream(a, up, z);
-  sepx::preference_grad(a, row_coef.data_ptr<float>(), cs());
+  sepx::preference_grad(a, a.lse + 2 * (int64_t)a.T, cs());
   return grad;
 }
 
@@ -306,15 +308,18 @@ std::vector<at::Tensor> router_balance_fwd(const at::Tensor& x, int64_t k, bool 
   a.blocks = sepx::router_balance_blocks(a.T, sms());
   at::Tensor w = at::empty({a.T, a.k}, f32), e = at::empty({a.T, a.k}, i32);
   at::Tensor loss = at::empty({}, f32), counts = at::empty({a.E}, i32), coef = at::empty({a.E}, f32);
-  at::Tensor part = at::empty({a.blocks, 2 * (int64_t)a.E + 1}, f32);
+  // scratch: parts of the loss, of the column sums and counts of each block, and a ticket
+  at::Tensor part = at::empty({2 * (int64_t)a.E + a.blocks * (2 * (int64_t)a.E + 1) + 1}, f32);
   a.topk_w = w.data_ptr<float>();
   a.topk_e = e.data_ptr<int>();
   a.loss = loss.data_ptr<float>();
   a.counts = counts.data_ptr<int>();
   a.coef = coef.data_ptr<float>();
-  a.part_p = part.data_ptr<float>();
+  a.part_l = reinterpret_cast<double*>(part.data_ptr<float>());
+  a.part_p = part.data_ptr<float>() + 2 * a.E;
   a.part_c = reinterpret_cast<int*>(a.part_p + (int64_t)a.blocks * a.E);
   a.part_n = a.part_c + (int64_t)a.blocks * a.E;
+  a.ticket = reinterpret_cast<unsigned int*>(a.part_n + a.blocks);
   sepx::router_balance_fwd(a, cs());
   return {w, e, loss, counts, coef};
 }
@@ -343,7 +348,7 @@ at::Tensor router_balance_bwd(const at::Tensor& x, const at::Tensor& topk_e, con
   }
   need_cuda(x, "router logits");
   const c10::cuda::CUDAGuard guard(x.device());
-  at::Tensor dx = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  at::Tensor dx = at::empty(x.sizes(), x.options());
   a.topk_e = topk_e.data_ptr<int>();
   a.coef = coef.data_ptr<float>();
   a.dx = dx.data_ptr();
@@ -458,7 +463,7 @@ struct PreferenceFn : torch::autograd::Function<PreferenceFn> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& z, const at::Tensor& labels,
                                const at::Tensor& offsets, const at::Tensor& ref_logp, double beta, double eps) {
     auto out = preference_fwd(z, labels, offsets, ref_logp, beta, eps, c10::nullopt);
-    ctx->save_for_backward({z, labels, offsets, out[3], out[4]});
+    ctx->save_for_backward({z, labels, offsets, out[3]});
     out.resize(3);
     ctx->mark_non_differentiable({out[1], out[2]});
     ctx->set_materialize_grads(false);
@@ -468,7 +473,7 @@ struct PreferenceFn : torch::autograd::Function<PreferenceFn> {
     at::Tensor g;
     if (up[0].defined()) {
       const auto s = ctx->get_saved_variables();
-      g = once(ctx, preference_grad(s[0], s[1], s[2], s[3], s[4], up[0]));
+      g = once(ctx, preference_grad(s[0], s[1], s[2], s[3], up[0]));
     }
     return {g, {}, {}, {}, {}, {}};
   }
@@ -528,4 +533,6 @@ void register_losses(pybind11::module& m) {
   m.def("distill_loss", &distill_loss);
   m.def("policy_loss", &policy_loss);
   m.def("preference_fwd", &preference_fwd);
+  m.def("router_balance_fwd", &router_balance_fwd);
+  m.def("router_balance_bwd", &router_balance_bwd);
 }

@@ -20,6 +20,8 @@ struct RouterBalanceArgs {
   int* part_c = nullptr;
   int* part_n = nullptr;
   int blocks = 0;
+  double* part_l = nullptr;          // [E] each expert's part of the loss
+  unsigned int* ticket = nullptr;    // [1], needs no value
   int* counts = nullptr;   // [E] tokens of the mask that chose each expert
   float* coef = nullptr;   // [E] d loss / d p of a token in the mask
   float* loss = nullptr;   // [1]

@@ -961,7 +961,10 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Voca
       a.logp[t] = (float)lp;
       if constexpr (OP == kOpLogp) {
         if (a.lse) reinterpret_cast<float2*>(a.lse)[t] = on ? make_float2(r.m, r.sum) : make_float2(0.f, 0.f);
-        if (a.ratio) a.ratio[t] = on ? (float)(lp - (double)a.ref_logp[t]) : 0.f;
+        if (a.ratio) {
+          a.ratio[t] = on ? (float)(lp - (double)a.ref_logp[t]) : 0.f;
+          a.row_coef[t] = 0.f;  // rows of no pair keep it
+        }
       } else {
         PolicyTerm o = {0.f, 0.f, 0.f};
         if (on)
@@ -993,26 +996,43 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Voca
 // ------------------------------------------------------------------------------------
 // rows in the loss, sums over rows, scaling
 // ------------------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) count_labels_kernel(const void* labels, bool is64, int T, int* count) {
+// One block: all labels, a load of several per thread in flight.
+__global__ void __launch_bounds__(1024) count_labels_kernel(const void* labels, bool is64, int T, int* count) {
+  __shared__ int red[32];
   int n = 0;
-  for (int t = blockIdx.x * blockDim.x + threadIdx.x; t < T; t += gridDim.x * blockDim.x)
-    n += load_id(labels, t, is64) >= 0;
+#pragma unroll 8
+  for (int t = threadIdx.x; t < T; t += 1024) n += load_id(labels, t, is64) >= 0;
   n = __reduce_add_sync(0xffffffffu, n);
-  if ((threadIdx.x & 31) == 0 && n) atomicAdd(count, n);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = n;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    n = __reduce_add_sync(0xffffffffu, red[threadIdx.x]);
+    if (threadIdx.x == 0) *count = n;
+  }
 }
-// one warp per row
-__global__ void __launch_bounds__(256) count_teacher_kernel(const void* ids, bool is64, const float* teacher, int T,
-                                                            int K, int* count) {
+// A warp per row. One block writes the count itself; several add to it (it is zeroed before;
+// whole numbers, so their order does not matter).
+__global__ void __launch_bounds__(1024) count_teacher_kernel(const void* ids, bool is64, const float* teacher, int T,
+                                                             int K, int* count) {
+  __shared__ int red[32];
   const int lane = threadIdx.x & 31;
-  const int warps = gridDim.x * (blockDim.x >> 5);
+  const int warps = gridDim.x * 32;
   int n = 0;
-  for (int t = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < T; t += warps) {
+  for (int t = (blockIdx.x * 1024 + threadIdx.x) >> 5; t < T; t += warps) {
     bool any = false;
     for (int k = lane; k < K && !any; k += 32)
       any = load_id(ids, (int64_t)t * K + k, is64) >= 0 && teacher[(int64_t)t * K + k] != -INFINITY;
     n += __any_sync(0xffffffffu, any) ? 1 : 0;
   }
-  if (lane == 0 && n) atomicAdd(count, n);
+  if (lane == 0) red[threadIdx.x >> 5] = n;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    n = __reduce_add_sync(0xffffffffu, red[threadIdx.x]);
+    if (threadIdx.x == 0) {
+      if (gridDim.x == 1) *count = n;
+      else atomicAdd(count, n);
+    }
+  }
 }
 
 // The gradient is already in its type: one more rounding where the loss's own gradient is
@@ -1040,6 +1060,7 @@ __global__ void __launch_bounds__(256) scale_grad_kernel(T* g, int64_t n, const 
 // two sums over whole sequences.
 __global__ void __launch_bounds__(256) preference_pairs_kernel(const PreferenceArgs a) {
   __shared__ double red[32];
+  __shared__ bool last;
   const int i = blockIdx.x;
   int lo[2], hi[2];
   double R[2];
@@ -1056,25 +1077,26 @@ __global__ void __launch_bounds__(256) preference_pairs_kernel(const PreferenceA
   const double neg = m > 0 ? sp : sp - m, pos = m > 0 ? sp + m : sp;  // softplus(-m), softplus(m)
   const double sig_neg = m > 0 ? e / (1.0 + e) : 1.0 / (1.0 + e), sig_pos = 1.0 - sig_neg;
   const double dm = ((double)a.eps * sig_pos - (1.0 - (double)a.eps) * sig_neg) / a.pairs;
-  if (threadIdx.x == 0) {
-    a.rewards[2 * i] = (float)R[0];
-    a.rewards[2 * i + 1] = (float)R[1];
-    a.pair_loss[i] = (float)((1.0 - (double)a.eps) * neg + (double)a.eps * pos);
-  }
   for (int s = 0; s < 2; ++s) {
     const float c = (float)((s ? -dm : dm) * (double)a.beta);
     for (int t = lo[s] + threadIdx.x; t < hi[s]; t += blockDim.x)
       if (load_id(a.labels, t, a.ids64) >= 0) a.row_coef[t] = c;
   }
-}
-
-// One block: the mean over pairs, in a fixed order.
-__global__ void __launch_bounds__(256) preference_mean_kernel(const float* __restrict__ x, int n, float* out) {
-  __shared__ double red[32];
+  // the mean over pairs: the last block adds them in their order
+  if (threadIdx.x == 0) {
+    a.rewards[2 * i] = (float)R[0];
+    a.rewards[2 * i + 1] = (float)R[1];
+    a.partial[i] = (1.0 - (double)a.eps) * neg + (double)a.eps * pos;
+    __threadfence();
+    last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
   double v = 0.0;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) v += x[i];
+  for (int p = threadIdx.x; p < a.pairs; p += blockDim.x) v += __ldcg(a.partial + p);
   v = block_sum_d(v, red);
-  if (threadIdx.x == 0) *out = (float)(v / max(n, 1));
+  if (threadIdx.x == 0) *a.loss = (float)(v / a.pairs);
 }
 
 // dz = up * row_coef * (onehot - softmax) from the saved log-sum-exp: one read, one write.
@@ -1228,10 +1250,14 @@ void launch_rows(const VocabLossArgs& a, int op, int num_sms, cudaStream_t st) {
 
 void vocab_count_rows(const VocabLossArgs& a, int op, int* count, cudaStream_t st) {
   if (a.T <= 0) return;
-  if (op == kOpDistill)
-    count_teacher_kernel<<<std::min((a.T + 7) / 8, 592), 256, 0, st>>>(a.ids, a.ids64, a.teacher, a.T, a.K, count);
-  else
-    count_labels_kernel<<<std::min((a.T + 255) / 256, 148), 256, 0, st>>>(a.labels, a.ids64, a.T, count);
+  if (op == kOpDistill) {
+    // a block of 32 rows at a time costs about 1.5 us per turn: more than 4 turns are split
+    const int blocks = a.T <= 128 ? 1 : std::min((a.T + 31) / 32, 148);
+    if (blocks > 1) cudaMemsetAsync(count, 0, sizeof(int), st);
+    count_teacher_kernel<<<blocks, 1024, 0, st>>>(a.ids, a.ids64, a.teacher, a.T, a.K, count);
+  } else {
+    count_labels_kernel<<<1, 1024, 0, st>>>(a.labels, a.ids64, a.T, count);
+  }
   check_launch("vocab_count_rows");
 }
 
@@ -1259,14 +1285,12 @@ void vocab_scale_grad(void* grad, int dtype, int64_t n, const float* up, int num
 }
 
 void preference_pairs(const PreferenceArgs& a, cudaStream_t st) {
-  if (a.pairs <= 0) return;
+  if (a.pairs <= 0) {  // a loss over nothing
+    cudaMemsetAsync(a.loss, 0, sizeof(float), st);
+    return;
+  }
   preference_pairs_kernel<<<a.pairs, 256, 0, st>>>(a);
   check_launch("preference_pairs");
-}
-
-void preference_loss_sum(const float* pair_loss, int pairs, float* loss, cudaStream_t st) {
-  preference_mean_kernel<<<1, 256, 0, st>>>(pair_loss, pairs, loss);
-  check_launch("preference_loss_sum");
 }
 
 void preference_grad(const VocabLossArgs& a, const float* row_coef, cudaStream_t st) {

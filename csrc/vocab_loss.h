@@ -50,13 +50,14 @@ struct VocabLossArgs {
   float* logp = nullptr;  // [T], kOpPolicy / kOpLogp
   float* kl = nullptr;    // [T], kOpPolicy
   float* ratio = nullptr;  // [T], kOpLogp: logp - ref_logp, 0 for rows not in the loss (optional)
+  float* row_coef = nullptr;  // [T], kOpLogp with ratio: set to 0
   float* lse = nullptr;    // [T, 2], kOpLogp: a reference m of the row and its sum of 2^((z - m) c2) (optional)
 };
 constexpr int kRowRecordBytes = 32;
 int vocab_finish_blocks(int T);
 
-// Rows in the loss: *count = number of rows with a label >= 0 (labels [T]), or with a
-// teacher entry (ids / teacher [T, K]). count must be zero before the call.
+// *count = rows in the loss: with a label >= 0 (labels [T]), or with a teacher entry (ids /
+// teacher [T, K]).
 void vocab_count_rows(const VocabLossArgs& a, int op, int* count, cudaStream_t st);
 void vocab_loss(const VocabLossArgs& a, int op, int num_sms, cudaStream_t st);
 // grad *= *up, in place; nothing is touched where *up is 1.
@@ -70,11 +71,12 @@ struct PreferenceArgs {
   int T = 0, pairs = 0;
   float beta = 0.f, eps = 0.f;
   float* rewards = nullptr;    // [2 * pairs]
-  float* pair_loss = nullptr;  // [pairs]
-  float* row_coef = nullptr;   // [T] d loss / d logp, zero-filled before the call
+  float* loss = nullptr;       // [1], the mean over pairs
+  float* row_coef = nullptr;   // [T] d loss / d logp; written for the pairs' rows with a label
+  double* partial = nullptr;   // [pairs] scratch
+  unsigned int* ticket = nullptr;  // [1], zero before the call
 };
 void preference_pairs(const PreferenceArgs& a, cudaStream_t st);
-void preference_loss_sum(const float* pair_loss, int pairs, float* loss, cudaStream_t st);
 // grad[t] = up * row_coef[t] * (onehot(labels[t]) - softmax(z[t])), zeros where row_coef is 0.
 void preference_grad(const VocabLossArgs& a, const float* row_coef, cudaStream_t st);
 
