@@ -59,8 +59,12 @@ sepx::VocabLossArgs vocab_args(const at::Tensor& z, const c10::optional<at::Tens
   a.dtype = vocab_dtype(z, "logits");
   a.T = (int)z.size(0);
   a.V = (int)z.size(1);
-  a.c2 = (float)(1.4426950408889634 / tau);
-  TORCH_CHECK(std::isfinite(a.c2) && a.c2 > 0, "temperature out of range");
+  // in two parts, the second above 0: a logit of -infinity has to stay one in both products
+  const double c2 = 1.4426950408889634 / tau;
+  a.c2 = (float)c2;
+  if ((double)a.c2 >= c2) a.c2 = std::nextafterf(a.c2, 0.f);
+  a.c2_lo = (float)(c2 - (double)a.c2);
+  TORCH_CHECK(std::isfinite(c2) && a.c2 > 1e-30f && a.c2 < 1e30f, "temperature out of range");
   a.tau = (float)tau;
   a.tau64 = tau;
   if (grad.has_value()) {

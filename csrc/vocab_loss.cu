@@ -216,27 +216,35 @@ __device__ __forceinline__ int64_t load_id(const void* p, int64_t i, bool is64) 
 }
 
 // ------------------------------------------------------------------------------------
-// Exponentials of a row: 2^(z c2 - M2), c2 = log2(e) / tau, M2 = the rounded product m c2 of
-// a reference m (the row's maximum, or near it). The same rounded M2 enters the sum, the
-// gradient and the logarithm, so its rounding cancels. Where m c2 leaves fp32 (rows whose
-// largest value is the type's lowest or highest), the difference z - m comes first.
+// Exponentials of a row: 2^(z c2 - M2), c2 = log2(e) / tau in two parts (the rounding of one
+// fp32 would show in log-probabilities: 1.3e-8 of a token's distance from the mean logit),
+// M2 = m c2 of a reference m (the row's maximum, or near it), rounded to a whole number: sums
+// against different references are joined by powers of two, exactly. Where m c2 leaves fp32
+// (rows whose largest value is the type's lowest or highest), the difference z - m comes
+// first.
 // ------------------------------------------------------------------------------------
 constexpr float kFarM2 = 1e37f;
+struct C2 {
+  float hi, lo;
+};
 struct Expo {
-  float c2, m, M2;
+  C2 c2;
+  float m, M2;
   bool far;
-  __device__ __forceinline__ Expo(float c2_, float m_) {
+  __device__ __forceinline__ Expo(C2 c2_, float m_) {
     c2 = c2_;
     m = m_;
-    M2 = __fmul_rn(m_, c2_);
+    M2 = rintf(m_ * c2.hi);
     far = !(fabsf(M2) <= kFarM2);
   }
-  __device__ __forceinline__ float arg(float z) const { return far ? (z - m) * c2 : fmaf(z, c2, -M2); }
+  __device__ __forceinline__ float arg(float z) const {
+    return far ? (z - m) * c2.hi : fmaf(z, c2.lo, fmaf(z, c2.hi, -M2));
+  }
   __device__ __forceinline__ float operator()(float z) const { return ex2(arg(z)); }
   // a sum against reference r, against this reference instead
   __device__ __forceinline__ float join(float r, float s) const {
     if (r == -INFINITY) return s;  // nothing yet: 0 (or NaN, which stays)
-    return s * ex2(far ? (r - m) * c2 : __fmul_rn(r, c2) - M2);
+    return s * ex2(far ? (r - m) * c2.hi : rintf(r * c2.hi) - M2);
   }
 };
 
@@ -251,7 +259,7 @@ __device__ __forceinline__ float max_of(const uint4& raw, float ref) {
 }
 // What the fast form z c2 + R adds for reference m: NaN (or infinity) where the sum has to
 // take the careful form.
-__device__ __forceinline__ float reference(float m, float c2) {
+__device__ __forceinline__ float reference(float m, C2 c2) {
   const Expo w(c2, m);
   return m == -INFINITY ? INFINITY : w.far ? __int_as_float(0x7fffffff) : -w.M2;
 }
@@ -260,7 +268,7 @@ __device__ __forceinline__ float reference(float m, float c2) {
 // whose reference moves, and a gradient with another phase, at a row's ends, or of a row
 // with a far reference. Out of line: they are rare, and inline they cost the usual path.
 template <typename T>
-__device__ __noinline__ float2 careful_sum(const uint4* v, int n, int step, float c2, float ref, float sum) {
+__device__ __noinline__ float2 careful_sum(const uint4* v, int n, int step, C2 c2, float ref, float sum) {
   float m = ref;
   for (int k = 0; k < n; ++k) m = max_of<T>(v[k * step], m);
   const Expo w(c2, m == -INFINITY ? 0.f : m);
@@ -274,7 +282,7 @@ __device__ __noinline__ float2 careful_sum(const uint4* v, int n, int step, floa
   return make_float2(m, sum);
 }
 template <typename T>
-__device__ __noinline__ void careful_store(const uint4* v, int n, int step, T* row, int V, int64_t e0, float c2, float m,
+__device__ __noinline__ void careful_store(const uint4* v, int n, int step, T* row, int V, int64_t e0, C2 c2, float m,
                                            float As) {
   constexpr int N = Elem<T>::N;
   const Expo w(c2, m);
@@ -301,7 +309,7 @@ __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile 
 enum RowState : int { kRowOff = 0, kRowOn = 1, kRowBad = 2 };
 
 struct RowRecord {
-  double base;    // distillation: sum P ln P - sum P (z - zref) c2 ln 2
+  double base;    // distillation: sum P (ln P - (z - zref) / tau)
   float m, sum;   // the row's reference and sum of exponentials
   float z;        // the token's logit; distillation: zref
   float weight;   // distillation: sum P
@@ -407,8 +415,8 @@ __device__ __forceinline__ int load_entries(const VocabLossArgs& a, int t, const
     const float lp = has ? (s.p[k] - top) / a.tau - lsum : 0.f;
     const float P = has ? expf(lp) : 0.f;
     s.p[k] = P;
-    if (P != 0.f) {  // P (ln P - (z - zref) / tau): the logits' exponent as the sum has it
-      base += (double)P * ((double)lp - ((double)s.z[k] - (double)zref) * ((double)a.c2 * 0.69314718055994530942));
+    if (P != 0.f) {  // P (ln P - (z - zref) / tau)
+      base += (double)P * ((double)lp - ((double)s.z[k] - (double)zref) / a.tau64);
       weight += P;
     }
   }
@@ -507,7 +515,7 @@ __global__ void __launch_bounds__(512) vocab_row_kernel(const VocabLossArgs a) {
 #pragma unroll
     for (int i = 0; i < N; ++i) mx = fmaxf(mx, o[i]);
   }
-  const Expo x(a.c2, block_max(mx, red));
+  const Expo x(C2{a.c2, a.c2_lo}, block_max(mx, red));
   for (int j = threadIdx.x; j < z.nv; j += blockDim.x) {
     float o[N];
     Elem<T>::unpack(z.load(j), o);
@@ -579,7 +587,7 @@ struct StreamShared {
 };
 
 // The row's reference and sum from all warps' pairs (one warp; the same bits in each).
-__device__ __forceinline__ void join_pairs(const float2* pairs, int n, float c2, int lane, float* m, float* sum) {
+__device__ __forceinline__ void join_pairs(const float2* pairs, int n, C2 c2, int lane, float* m, float* sum) {
   float mx = -INFINITY, v = 0.f;
   for (int i = lane; i < n; i += 32) mx = fmaxf(mx, pairs[i].x);
   mx = warp_max(mx);
@@ -748,7 +756,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
       for (int t = cluster; t < a.T; t += clusters) {
         if (!wait(&sh.dense_done[e], lap)) break;
         if (a.grad && sh.token[e].state != kRowOff) {  // the entries' values replace the dense ones
-          const Expo x(a.c2, sh.factor[e][2]);
+          const Expo x(C2{a.c2, a.c2_lo}, sh.factor[e][2]);
           const float A = sh.factor[e][0], As = sh.factor[e][1];
           const Entries s = entries(e);
           const RowVec<T> z = row_z(t);
@@ -796,7 +804,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
       // vector takes no maximum.
       float ref = -INFINITY, sum = 0.f;
       F2 nR2 = f2(0.f, 0.f);
-      const F2 cc = f2(a.c2, a.c2);
+      const F2 cc = f2(a.c2, a.c2), cl = f2(a.c2_lo, a.c2_lo);
       for (int left = mine, first = 1, end = j1 - j0; end > 0; left -= Cfg::VPT, first = 0, end -= kPieceVecs) {
         if (!wait(&sh.full[slot], turn)) { ok = false; break; }
         const uint4* piece = reinterpret_cast<const uint4*>(ring + (size_t)slot * kPieceBytes) + tid;
@@ -807,7 +815,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
           if (first) {
 #pragma unroll
             for (int v = 0; v < Cfg::VPT; ++v) ref = max_of<T>(raw[v], ref);
-            const float R = reference(ref, a.c2);
+            const float R = reference(ref, C2{a.c2, a.c2_lo});
             nR2 = f2(R, R);
           }
           F2 acc[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
@@ -816,7 +824,8 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
             float o[N];
             Elem<T>::unpack(raw[v], o);
 #pragma unroll
-            for (int i = 0; i < N; i += 2) acc[(i >> 1) & 1] = add2(acc[(i >> 1) & 1], ex2_2(fma2(f2(o[i], o[i + 1]), cc, nR2)));
+            for (int i = 0; i < N; i += 2) acc[(i >> 1) & 1] = add2(acc[(i >> 1) & 1], 
+                                                        ex2_2(fma2(f2(o[i], o[i + 1]), cl, fma2(f2(o[i], o[i + 1]), cc, nR2))));
           }
           float ax, ay;
           split(add2(acc[0], acc[1]), ax, ay);
@@ -824,14 +833,14 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
           if (s1 <= 1.0995e12f) {
             sum = s1;
           } else {  // NaN too
-            const float2 r = careful_sum<T>(piece, Cfg::VPT, Cfg::Lanes, a.c2, ref, first ? 0.f : sum);
+            const float2 r = careful_sum<T>(piece, Cfg::VPT, Cfg::Lanes, C2{a.c2, a.c2_lo}, ref, first ? 0.f : sum);
             ref = r.x;
             sum = r.y;
-            const float R = reference(ref, a.c2);
+            const float R = reference(ref, C2{a.c2, a.c2_lo});
             nR2 = f2(R, R);
           }
         } else if (left > 0) {  // the last piece, partly filled
-          const float2 r = careful_sum<T>(piece, min(left, Cfg::VPT), Cfg::Lanes, a.c2, ref, sum);
+          const float2 r = careful_sum<T>(piece, min(left, Cfg::VPT), Cfg::Lanes, C2{a.c2, a.c2_lo}, ref, sum);
           ref = r.x;
           sum = r.y;
         }
@@ -849,7 +858,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
       // may only leave once this block has all pairs of row x - 1.
       if (!a.grad && x > 0 && !wait(&sh.pairs_full[(x - 1) & 1], (x - 1) >> 1)) break;
       const float mw = warp_max(ref);
-      sum = warp_sum(Expo(a.c2, mw).join(ref, sum));
+      sum = warp_sum(Expo(C2{a.c2, a.c2_lo}, mw).join(ref, sum));
       if (C == 1) {
         if (lane == 0) {
           sh.pairs[x & 1][warp] = make_float2(mw, sum);
@@ -864,14 +873,14 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
       if (a.grad || warp == 0) {
         if (!wait(&sh.pairs_full[x & 1], x >> 1)) break;
         float m, tot;
-        join_pairs(sh.pairs[x & 1], C * CW, a.c2, lane, &m, &tot);
+        join_pairs(sh.pairs[x & 1], C * CW, C2{a.c2, a.c2_lo}, lane, &m, &tot);
         if (rank == 0 && warp == 0 && lane == 0) {
           RowRecord* rec = reinterpret_cast<RowRecord*>(a.records) + t;
           rec->m = m;
           rec->sum = tot;
         }
         if (a.grad) {  // second pass
-        const Expo w(a.c2, m);
+        const Expo w(C2{a.c2, a.c2_lo}, m);
         const float A = row_factor<OP>(a, token, w, tot, factor), As = A / tot;
         if (OP == kOpDistill && warp == 0 && lane == 0) {
           sh.factor[e][0] = A;
@@ -904,7 +913,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
               *reinterpret_cast<uint4*>(gp + v * Cfg::Lanes * N) = Elem<T>::pack(o);
             }
           } else if (left > 0) {
-            careful_store<T>(piece, min(left, Cfg::VPT), Cfg::Lanes, g.p, a.V, z.first(base + tid), a.c2, m, As);
+            careful_store<T>(piece, min(left, Cfg::VPT), Cfg::Lanes, g.p, a.V, z.first(base + tid), C2{a.c2, a.c2_lo}, m, As);
           }
           if (n == own_piece) g.p[token.id] = Elem<T>::t(As * w(token.z) - A);
           __syncwarp();
@@ -947,10 +956,10 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Voca
   float loss = 0.f;
   if (t < a.T) {
     const RowRecord r = reinterpret_cast<const RowRecord*>(a.records)[t];
-    const Expo x(a.c2, r.m);
+    const Expo x(C2{a.c2, a.c2_lo}, r.m);
     double lp = 0.0;  // ln q of the token (of the entry that zref is from)
     if (r.state == kRowOn)
-      lp = (x.far ? ((double)r.z - (double)r.m) * (double)a.c2 : (double)r.z * (double)a.c2 - (double)x.M2) * ln2 -
+      lp = (x.far ? ((double)r.z - (double)r.m) / a.tau64 : (double)r.z / a.tau64 - (double)x.M2 * ln2) -
            log((double)r.sum);
     if constexpr (OP == kOpDistill) {
       if (r.state == kRowOn) loss = (float)((double)a.tau * a.tau * (r.base - (double)r.weight * lp));
@@ -1114,7 +1123,7 @@ __global__ void __launch_bounds__(256) preference_grad_kernel(const VocabLossArg
   const bool on = label >= 0 && t >= a.offsets[0] && t < a.offsets[a.num_seq];
   const float A = on ? -coef * *a.up : 0.f;
   const float2 l = reinterpret_cast<const float2*>(a.lse)[t];  // the row's maximum and sum
-  const Expo x(a.c2, l.x);
+  const Expo x(C2{a.c2, a.c2_lo}, l.x);
   const float As = A / l.y;
   for (int j = j0 + threadIdx.x; j < j1; j += blockDim.x) {
     float o[N];
