@@ -265,8 +265,8 @@ __device__ __forceinline__ float reference(float m, C2 c2) {
 }
 
 // The careful forms of the two passes over n vectors `step` apart in shared memory: a sum
-// whose reference moves, and a gradient with another phase, at a row's ends, or of a row
-// with a far reference. Out of line: they are rare, and inline they cost the usual path.
+// whose reference moves, and a vector of a gradient with another phase, at a row's ends, or of
+// a row with a far reference. Out of line: they are rare, and inline they cost the usual path.
 template <typename T>
 __device__ __noinline__ float2 careful_sum(const uint4* v, int n, int step, C2 c2, float ref, float sum) {
   float m = ref;
@@ -282,21 +282,40 @@ __device__ __noinline__ float2 careful_sum(const uint4* v, int n, int step, C2 c
   return make_float2(m, sum);
 }
 template <typename T>
-__device__ __noinline__ void careful_store(const uint4* v, int n, int step, T* row, int V, int64_t e0, C2 c2, float m,
-                                           float As) {
+__device__ __noinline__ void careful_store(const uint4* v, T* row, int V, int64_t e0, C2 c2, float m, float As) {
   constexpr int N = Elem<T>::N;
   const Expo w(c2, m);
   const RowVec<T> g(row, V);
-  for (int k = 0; k < n; ++k) {
-    float o[N];
-    Elem<T>::unpack(v[k * step], o);
+  float o[N];
+  Elem<T>::unpack(*v, o);
 #pragma unroll
-    for (int i = 0; i < N; ++i) o[i] = As * w(o[i]);
-    g.store(e0 + (int64_t)k * step * N, o);
+  for (int i = 0; i < N; ++i) o[i] = As * w(o[i]);
+  g.store(e0, o);
+}
+// Bounded waits, out of line. The usual one sleeps in the barrier (polls of a waiting warp take
+// issue slots from the working ones); the exchange of a row's sums, where every cycle
+// counts, polls.
+__device__ __noinline__ bool wait_asleep(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  const uint64_t t0 = globaltimer_ns();
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)  // ns
+        : "memory");
+    if (ok) return true;
+    if (*abort) return false;
+    if (globaltimer_ns() - t0 > 2000000000ull) {
+      *abort = 1;
+      return false;
+    }
   }
 }
-__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort, nullptr, 2000000000ull)) != 0;
+__device__ __noinline__ bool wait_awake(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return mbar_wait_bounded(bar, parity, abort, nullptr, 2000000000ull);
 }
 
 // ------------------------------------------------------------------------------------
@@ -555,8 +574,9 @@ __global__ void __launch_bounds__(512) vocab_row_kernel(const VocabLossArgs a) {
 //   load warp       bulk copies of whole vectors; the partial vectors at a row's ends come
 //                   from the prepare warp
 //   prepare warp    tokens (8 rows at a time) or teacher entries of the rows to come
-//   fix warp        distillation: the gradient at the entries' ids, once the block's dense
-//                   part is written (a single token is set by the thread that owns its vector)
+//   join warp       the row's sum from all warps' parts and the factor of its gradient;
+//                   distillation: the gradient at the entries' ids, once the block's dense part
+//                   is written (a single token is set by the thread that owns its vector)
 // Partial sums travel as (reference, sum) pairs of each warp, with asynchronous stores that
 // complete on the receiver's mbarrier. Pair buffers alternate: a warp sends row r + 2 after it
 // has row r + 1 of every warp, and each of those left after its block had all of row r.
@@ -578,10 +598,10 @@ constexpr int kTokens = 16;  // rows between the prepare warp and the others (to
 struct StreamShared {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
   uint64_t ent_full[kTokens], ent_done[kTokens], dense_done[kTokens];
-  uint64_t pairs_full[2];
+  uint64_t pairs_full[2], factor_full[2];
   uint4 edge[kTokens][2];  // a row's first and last vector, where they are partial
   Token token[kTokens];
-  float factor[kTokens][4];  // A, A / sum, reference
+  float factor[2][4];  // A, A / sum, reference
   float2 pairs[2][kMaxCluster * kMaxConsumers];
   int abort;
 };
@@ -619,20 +639,30 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
     }
     for (int i = 0; i < rows_ahead; ++i) {
       mbar_init(&sh.ent_full[i], 1);
-      // the load warp, and the last reader: the consumers, or the fix warp after them
-      mbar_init(&sh.ent_done[i], OP == kOpDistill ? 2 : CW + 1);
+      // the load and join warps, and the consumers (distillation: the join warp after them)
+      mbar_init(&sh.ent_done[i], OP == kOpDistill ? 2 : CW + 2);
       mbar_init(&sh.dense_done[i], CW);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(&sh.pairs_full[i], C == 1 ? CW : 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sh.pairs_full[i], C == 1 ? CW : 1);
+      mbar_init(&sh.factor_full[i], 1);
+    }
     sh.abort = 0;
     fence_barrier_init();
     if (blockIdx.x == 0) *a.ticket = 0;  // for the kernel that forms the outputs
   }
   __syncthreads();
   if (C > 1) cluster_sync();  // the other blocks' barriers are ready too
-  auto wait = [&](uint64_t* bar, int phase) {  // all lanes of a warp, with one answer
-    const bool now = __all_sync(0xffffffffu, mbar_try_wait(bar, (uint32_t)phase & 1u));
-    return now || wait_slow(bar, (uint32_t)phase & 1u, abort);
+  // all lanes of a warp, with one answer
+  auto wait = [&](uint64_t* bar, int phase) {
+    const uint32_t parity = (uint32_t)phase & 1u;
+    return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) ||
+           __all_sync(0xffffffffu, wait_asleep(bar, parity, abort));
+  };
+  auto wait_exchange = [&](uint64_t* bar, int phase) {
+    const uint32_t parity = (uint32_t)phase & 1u;
+    return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) ||
+           __all_sync(0xffffffffu, wait_awake(bar, parity, abort));
   };
   const int log2c = 31 - __clz(C);
   // this block's vectors of row t
@@ -730,7 +760,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
         if (!__any_sync(0xffffffffu, mine)) break;
         const int e = (g0 + lane) % kTokens;
         bool ok = true;
-        if (mine) ok = mbar_wait_bounded(&sh.ent_done[e], (uint32_t)(((g0 + lane) / kTokens) & 1) ^ 1u, abort, nullptr, 2000000000ull);
+        if (mine) ok = wait_asleep(&sh.ent_done[e], (uint32_t)(((g0 + lane) / kTokens) & 1) ^ 1u, abort);
         if (!__all_sync(0xffffffffu, ok)) break;
         if (mine) {
           const RowVec<T> z = row_z((int)t);
@@ -750,14 +780,40 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
       }
     }
   } else if (warp == CW + 2) {
-    // -------------------------------- fix --------------------------------
-    if constexpr (OP == kOpDistill) {
-      int e = 0, lap = 0;
-      for (int t = cluster; t < a.T; t += clusters) {
+    // ---------------------------- join and fix ----------------------------
+    const float factor = loss_factor(a);
+    int e = 0, lap = 0, x = 0;
+    for (int t = cluster; t < a.T; t += clusters) {
+      if (!wait(&sh.ent_full[e], lap)) break;
+      const Token token = sh.token[e];
+      float m = 0.f, A = 0.f, As = 0.f;
+      if (token.state != kRowOff) {
+        if (C > 1 && lane == 0) mbar_arrive_expect_tx(&sh.pairs_full[x & 1], (uint32_t)(C * CW) * 8u);
+        __syncwarp();
+        if (!wait_exchange(&sh.pairs_full[x & 1], x >> 1)) break;
+        float sum;
+        join_pairs(sh.pairs[x & 1], C * CW, C2{a.c2, a.c2_lo}, lane, &m, &sum);
+        if (a.grad) {
+          A = row_factor<OP>(a, token, Expo(C2{a.c2, a.c2_lo}, m), sum, factor);
+          As = A / sum;
+        }
+        if (lane == 0) {
+          sh.factor[x & 1][0] = A;
+          sh.factor[x & 1][1] = As;
+          sh.factor[x & 1][2] = m;
+          mbar_arrive(&sh.factor_full[x & 1]);
+          if (rank == 0) {
+            RowRecord* rec = reinterpret_cast<RowRecord*>(a.records) + t;
+            rec->m = m;
+            rec->sum = sum;
+          }
+        }
+        ++x;
+      }
+      if constexpr (OP == kOpDistill) {
         if (!wait(&sh.dense_done[e], lap)) break;
-        if (a.grad && sh.token[e].state != kRowOff) {  // the entries' values replace the dense ones
-          const Expo x(C2{a.c2, a.c2_lo}, sh.factor[e][2]);
-          const float A = sh.factor[e][0], As = sh.factor[e][1];
+        if (a.grad && token.state != kRowOff) {  // the entries' values replace the dense ones
+          const Expo w(C2{a.c2, a.c2_lo}, m);
           const Entries s = entries(e);
           const RowVec<T> z = row_z(t);
           int j0, j1;
@@ -765,100 +821,191 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
           const int64_t e0 = z.first(j0), e1 = z.first(j1);
           T* g = reinterpret_cast<T*>(a.grad) + (int64_t)t * a.grad_stride;
           for (int k = lane; k < a.K; k += 32)
-            if (s.id[k] >= 0 && s.id[k] >= e0 && s.id[k] < e1) g[s.id[k]] = Elem<T>::t(As * x(s.z[k]) - A * weight_of(s, s.id[k]));
+            if (s.id[k] >= 0 && s.id[k] >= e0 && s.id[k] < e1)
+              g[s.id[k]] = Elem<T>::t(As * w(s.z[k]) - A * weight_of(s, s.id[k]));
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh.ent_done[e]);
-        __syncwarp();
-        next_entry(e, lap);
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.ent_done[e]);
+      __syncwarp();
+      next_entry(e, lap);
     }
   } else {
     // ---------------------------- sum and gradient ----------------------------
+    // A row's sum is complete some 2500 cycles before its factor is back from the other
+    // warps and blocks: meanwhile the sum of the next row begins, over the pieces that are
+    // there already.
+    constexpr int kAhead = 3;
     const int tid = threadIdx.x;
-    const float factor = loss_factor(a);
-    int slot = 0, turn = 0, x = 0, e = 0, lap = 0;
-    bool ok = true;
-    for (int t = cluster; t < a.T && ok; t += clusters) {
-      if (!wait(&sh.ent_full[e], lap)) break;
-      const Token token = sh.token[e];
-      const RowVec<T> z = row_z(t);
-      const RowVec<T> g(reinterpret_cast<T*>(a.grad) + (a.grad ? (int64_t)t * a.grad_stride : 0), a.V);
-      int j0, j1;
-      part(z, &j0, &j1);
-      if (token.state == kRowOff) {
+    uint4 none;  // a vector of -infinity
+    {
+      float o[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = -INFINITY;
+      none = Elem<T>::pack(o);
+    }
+    const C2 c2 = {a.c2, a.c2_lo};
+    const F2 cc = f2(a.c2, a.c2), cl = f2(a.c2_lo, a.c2_lo);
+    int slot = 0, turn = 0, grad_slot = 0, e = 0, lap = 0, x = 0;
+    // the row that is summed: done of np pieces
+    int t = cluster, np = 0, done = 0, part_n = 0;
+    bool open = false;
+    float ref = -INFINITY, sum = 0.f;
+    F2 nR2 = f2(0.f, 0.f);
+    // the row that waits for its factor
+    int tg = -1, eg = 0;
+    for (;;) {
+      while (!open && t < a.T) {
+        if (tg >= 0) {
+          // a row's gradient is still owed, and the entries to come may wait for its own
+          if (!__all_sync(0xffffffffu, mbar_test_wait(&sh.ent_full[e], (uint32_t)lap))) break;
+        } else if (!wait(&sh.ent_full[e], lap)) {
+          goto out;
+        }
+        const RowVec<T> z = row_z(t);
+        int j0, j1;
+        part(z, &j0, &j1);
+        if (sh.token[e].state != kRowOff) {
+          open = true;
+          part_n = j1 - j0;
+          np = (part_n + kPieceVecs - 1) / kPieceVecs;
+          done = 0;
+          ref = -INFINITY;
+          sum = 0.f;
+          break;
+        }
         if (a.grad) {
+          const RowVec<T> g(reinterpret_cast<T*>(a.grad) + (int64_t)t * a.grad_stride, a.V);
           const float o[N] = {};
           for (int j = j0 + tid; j < j1; j += Cfg::Lanes) g.store(z.first(j), o);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(OP == kOpDistill ? &sh.dense_done[e] : &sh.ent_done[e]);
         next_entry(e, lap);
-        continue;
+        t += clusters;
       }
-      if (C > 1 && warp == 0 && lane == 0) mbar_arrive_expect_tx(&sh.pairs_full[x & 1], (uint32_t)(C * CW) * 8u);
-      const int slot0 = slot;
-      const int mine = (j1 - j0 - tid + Cfg::Lanes - 1) / Cfg::Lanes;  // this thread's vectors (or < 1)
-      // Sum against a reference that is the maximum of the thread's first vectors: the sum may
-      // grow to 2^40 before the reference is moved, which costs fp32 nothing, so the usual
-      // vector takes no maximum.
-      float ref = -INFINITY, sum = 0.f;
-      F2 nR2 = f2(0.f, 0.f);
-      const F2 cc = f2(a.c2, a.c2), cl = f2(a.c2_lo, a.c2_lo);
-      for (int left = mine, first = 1, end = j1 - j0; end > 0; left -= Cfg::VPT, first = 0, end -= kPieceVecs) {
-        if (!wait(&sh.full[slot], turn)) { ok = false; break; }
-        const uint4* piece = reinterpret_cast<const uint4*>(ring + (size_t)slot * kPieceBytes) + tid;
-        if (end >= kPieceVecs) {
+      if (open) {
+        // Sum against a reference that is the maximum of the thread's first vectors: the sum
+        // may grow to 2^40 before the reference is moved, which costs fp32 nothing, so the
+        // usual vector takes no maximum.
+        const int stop = tg >= 0 ? min(np, done + kAhead) : np;
+        for (; done < stop; ++done) {
+          if (tg >= 0) {
+            if (!__all_sync(0xffffffffu, mbar_test_wait(&sh.full[slot], (uint32_t)turn))) break;
+          } else if (!wait(&sh.full[slot], turn)) {
+            goto out;
+          }
+          const int end = part_n - done * kPieceVecs;                // vectors left
+          const int left = (end - tid + Cfg::Lanes - 1) / Cfg::Lanes;  // of them this thread's (or < 1)
+          const uint4* piece = reinterpret_cast<const uint4*>(ring + (size_t)slot * kPieceBytes) + tid;
           uint4 raw[Cfg::VPT];
+          if (end >= kPieceVecs) {
 #pragma unroll
-          for (int v = 0; v < Cfg::VPT; ++v) raw[v] = piece[v * Cfg::Lanes];
-          if (first) {
+            for (int v = 0; v < Cfg::VPT; ++v) raw[v] = piece[v * Cfg::Lanes];
+          } else {  // the last piece, partly filled
+#pragma unroll
+            for (int v = 0; v < Cfg::VPT; ++v) raw[v] = v < left ? piece[v * Cfg::Lanes] : none;
+          }
+          if (done == 0) {
 #pragma unroll
             for (int v = 0; v < Cfg::VPT; ++v) ref = max_of<T>(raw[v], ref);
-            const float R = reference(ref, C2{a.c2, a.c2_lo});
+            const float R = reference(ref, c2);
             nR2 = f2(R, R);
           }
           F2 acc[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
 #pragma unroll
           for (int v = 0; v < Cfg::VPT; ++v) {
+            if (v > 0 && end <= v * Cfg::Lanes) break;  // nothing left for any thread
             float o[N];
             Elem<T>::unpack(raw[v], o);
 #pragma unroll
-            for (int i = 0; i < N; i += 2) acc[(i >> 1) & 1] = add2(acc[(i >> 1) & 1], 
-                                                        ex2_2(fma2(f2(o[i], o[i + 1]), cl, fma2(f2(o[i], o[i + 1]), cc, nR2))));
+            for (int i = 0; i < N; i += 2) {
+              const F2 z2 = f2(o[i], o[i + 1]);
+              acc[(i >> 1) & 1] = add2(acc[(i >> 1) & 1], ex2_2(fma2(z2, cl, fma2(z2, cc, nR2))));
+            }
           }
           float ax, ay;
           split(add2(acc[0], acc[1]), ax, ay);
           const float s1 = sum + (ax + ay);
           if (s1 <= 1.0995e12f) {
             sum = s1;
-          } else {  // NaN too
-            const float2 r = careful_sum<T>(piece, Cfg::VPT, Cfg::Lanes, C2{a.c2, a.c2_lo}, ref, first ? 0.f : sum);
+          } else if (left > 0) {  // NaN too
+            const float2 r = careful_sum<T>(piece, min(left, Cfg::VPT), Cfg::Lanes, c2, done == 0 ? -INFINITY : ref, sum);
             ref = r.x;
             sum = r.y;
-            const float R = reference(ref, C2{a.c2, a.c2_lo});
+            const float R = reference(ref, c2);
             nR2 = f2(R, R);
           }
-        } else if (left > 0) {  // the last piece, partly filled
-          const float2 r = careful_sum<T>(piece, min(left, Cfg::VPT), Cfg::Lanes, C2{a.c2, a.c2_lo}, ref, sum);
-          ref = r.x;
-          sum = r.y;
-        }
-        if (!a.grad) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.empty[slot]);
-        }
-        if (++slot == slots) {
-          slot = 0;
-          turn ^= 1;
+          if (!a.grad) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.empty[slot]);
+          }
+          if (++slot == slots) {
+            slot = 0;
+            turn ^= 1;
+          }
         }
       }
-      if (!ok) break;
+      if (tg >= 0) {
+        const int xg = x - 1;
+        if (!wait_exchange(&sh.factor_full[xg & 1], xg >> 1)) goto out;
+        const float As = sh.factor[xg & 1][1], m = sh.factor[xg & 1][2];
+        const Expo w(c2, m);
+        const RowVec<T> z = row_z(tg);
+        const RowVec<T> g(reinterpret_cast<T*>(a.grad) + (int64_t)tg * a.grad_stride, a.V);
+        int j0, j1;
+        part(z, &j0, &j1);
+        const F2 nM2 = f2(-w.M2, -w.M2), As2 = f2(As, As);
+        const bool plain = g.a == z.a && !w.far;
+        // whole vectors of this part: pieces within them take the straight path
+        const int lo = z.full(0) ? 0 : 1, hi = z.full(z.nv - 1) ? z.nv : z.nv - 1;
+        T* gp = g.p + z.first(j0 + tid);
+        for (int base = j0; base < j1; base += kPieceVecs, gp += kPieceVecs * N) {
+          const uint4* piece = reinterpret_cast<const uint4*>(ring + (size_t)grad_slot * kPieceBytes) + tid;
+          auto grad_vec = [&](const uint4& raw, int v) {
+            float o[N];
+            Elem<T>::unpack(raw, o);
+#pragma unroll
+            for (int i = 0; i < N; i += 2)
+              split(mul2(As2, ex2_2(fma2(f2(o[i], o[i + 1]), cc, nM2))), o[i], o[i + 1]);
+            *reinterpret_cast<uint4*>(gp + v * Cfg::Lanes * N) = Elem<T>::pack(o);
+          };
+          if (plain && base >= lo && base + kPieceVecs <= min(hi, j1)) {
+            uint4 raw[Cfg::VPT];
+#pragma unroll
+            for (int v = 0; v < Cfg::VPT; ++v) raw[v] = piece[v * Cfg::Lanes];
+#pragma unroll
+            for (int v = 0; v < Cfg::VPT; ++v) grad_vec(raw[v], v);
+          } else {  // a row's end in this piece, another phase, or a far reference
+#pragma unroll 1
+            for (int v = 0; v < Cfg::VPT; ++v) {
+              const int j = base + tid + v * Cfg::Lanes;
+              if (j >= j1) break;
+              if (plain && j >= lo && j < hi) grad_vec(piece[v * Cfg::Lanes], v);
+              else careful_store<T>(piece + v * Cfg::Lanes, g.p, a.V, z.first(j), c2, m, As);
+            }
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.empty[grad_slot]);
+          if (++grad_slot == slots) grad_slot = 0;
+        }
+        if constexpr (OP != kOpDistill) {  // the token's element, from the thread that wrote its vector
+          const Token token = sh.token[eg];
+          const int own = (int)(((int64_t)token.id + z.a) / N) - j0;
+          if (own >= 0 && own < j1 - j0 && own % Cfg::Lanes == tid)
+            g.p[token.id] = Elem<T>::t(As * w(token.z) - sh.factor[xg & 1][0]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(OP == kOpDistill ? &sh.dense_done[eg] : &sh.ent_done[eg]);
+        tg = -1;
+        continue;
+      }
+      if (!open) break;
       // Without a gradient nothing else makes a warp wait for the row before: a pair of row x
-      // may only leave once this block has all pairs of row x - 1.
-      if (!a.grad && x > 0 && !wait(&sh.pairs_full[(x - 1) & 1], (x - 1) >> 1)) break;
+      // may only leave once this block has joined row x - 1.
+      if (!a.grad && x > 0 && !wait(&sh.factor_full[(x - 1) & 1], (x - 1) >> 1)) goto out;
       const float mw = warp_max(ref);
-      sum = warp_sum(Expo(C2{a.c2, a.c2_lo}, mw).join(ref, sum));
+      sum = warp_sum(Expo(c2, mw).join(ref, sum));
       if (C == 1) {
         if (lane == 0) {
           sh.pairs[x & 1][warp] = make_float2(mw, sum);
@@ -870,63 +1017,18 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
         st_async_f2(to, mw, sum, bar);
       }
       __syncwarp();
-      if (a.grad || warp == 0) {
-        if (!wait(&sh.pairs_full[x & 1], x >> 1)) break;
-        float m, tot;
-        join_pairs(sh.pairs[x & 1], C * CW, C2{a.c2, a.c2_lo}, lane, &m, &tot);
-        if (rank == 0 && warp == 0 && lane == 0) {
-          RowRecord* rec = reinterpret_cast<RowRecord*>(a.records) + t;
-          rec->m = m;
-          rec->sum = tot;
-        }
-        if (a.grad) {  // second pass
-        const Expo w(C2{a.c2, a.c2_lo}, m);
-        const float A = row_factor<OP>(a, token, w, tot, factor), As = A / tot;
-        if (OP == kOpDistill && warp == 0 && lane == 0) {
-          sh.factor[e][0] = A;
-          sh.factor[e][1] = As;
-          sh.factor[e][2] = m;
-        }
-        const F2 nM2 = f2(-w.M2, -w.M2), As2 = f2(As, As);
-        const bool plain = g.a == z.a && !w.far;
-        // whole vectors of this part: pieces within them take the straight path
-        const int lo = z.full(0) ? 0 : 1, hi = z.full(z.nv - 1) ? z.nv : z.nv - 1;
-        // the token's element belongs to the thread that writes its vector
-        const int own = OP == kOpDistill ? -1 : (int)(((int64_t)token.id + z.a) / N) - j0;
-        const bool own_mine = own >= 0 && own < j1 - j0 && own % Cfg::Lanes == tid;
-        const int own_piece = own_mine ? own / kPieceVecs : -1;
-        T* gp = g.p + z.first(j0 + tid);
-        int sl = slot0, left = mine;
-        for (int base = j0, n = 0; base < j1; base += kPieceVecs, ++n, left -= Cfg::VPT, gp += kPieceVecs * N) {
-          const uint4* piece = reinterpret_cast<const uint4*>(ring + (size_t)sl * kPieceBytes) + tid;
-          if (plain && base >= lo && base + kPieceVecs <= min(hi, j1)) {
-            uint4 raw[Cfg::VPT];
-#pragma unroll
-            for (int v = 0; v < Cfg::VPT; ++v) raw[v] = piece[v * Cfg::Lanes];
-#pragma unroll
-            for (int v = 0; v < Cfg::VPT; ++v) {
-              float o[N];
-              Elem<T>::unpack(raw[v], o);
-#pragma unroll
-              for (int i = 0; i < N; i += 2)
-                split(mul2(As2, ex2_2(fma2(f2(o[i], o[i + 1]), cc, nM2))), o[i], o[i + 1]);
-              *reinterpret_cast<uint4*>(gp + v * Cfg::Lanes * N) = Elem<T>::pack(o);
-            }
-          } else if (left > 0) {
-            careful_store<T>(piece, min(left, Cfg::VPT), Cfg::Lanes, g.p, a.V, z.first(base + tid), C2{a.c2, a.c2_lo}, m, As);
-          }
-          if (n == own_piece) g.p[token.id] = Elem<T>::t(As * w(token.z) - A);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.empty[sl]);
-          if (++sl == slots) sl = 0;
-        }
-        }
+      if (a.grad) {
+        tg = t;
+        eg = e;
+      } else if (lane == 0) {
+        mbar_arrive(OP == kOpDistill ? &sh.dense_done[e] : &sh.ent_done[e]);
       }
       ++x;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(OP == kOpDistill ? &sh.dense_done[e] : &sh.ent_done[e]);
       next_entry(e, lap);
+      t += clusters;
+      open = false;
     }
+  out:;
   }
   if (*abort) {  // copies in flight land long before this
     const uint64_t t0 = globaltimer_ns();

@@ -562,3 +562,45 @@ def test_gradient_reaches_a_leaf_behind_other_operations(i):
         _three(leaf, i).backward()
     (once,) = torch.autograd.grad(_three(leaf, i), leaf)
     assert torch.equal(leaf.grad, 2 * once)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [300, 9000, 40001, 151936])
+@pytest.mark.parametrize("pattern", ["runs", "scattered", "ends"])
+def test_many_rows_out_of_the_loss(V, pattern):
+    """Long runs of rows that are not in the loss between rows that are, over several rows
+    per block: all losses equal those of the remaining rows alone."""
+    from spec_ep.ops.loss import clipped_policy_loss, preference_loss, topk_distill_loss
+
+    T = 1500 if V > 100000 else 3000
+    g = torch.Generator(device="cuda").manual_seed(V)
+    z = torch.randn(T, V, generator=g, device="cuda").bfloat16()
+    r = torch.arange(T, device="cuda")
+    on = {"runs": (r // 700) % 2 == 1, "scattered": torch.rand(T, generator=g, device="cuda") < 0.15,
+          "ends": (r < 3) | (r >= T - 2)}[pattern]
+    z[~on] = math.nan
+    z.requires_grad_()
+    zk = z.detach()[on].requires_grad_()
+    n = int(on.sum())
+    y = torch.where(on, (r * 17) % V, -1)
+    old, adv = torch.full((T,), -9.0, device="cuda"), 1.0 + (r % 5).float()
+    ids = torch.where(on[:, None], (r[:, None] * 31 + torch.arange(6, device="cuda") * 7) % V, -1)
+    big = torch.where(on[:, None], (r[:, None] + torch.arange(300, device="cuda")) % V, -1)
+    t6, t300 = torch.linspace(1, 0, 6, device="cuda"), torch.linspace(2, 0, 300, device="cuda")
+    off, offk = ([0, T // 2, T], [0, int(on[:T // 2].sum()), n])
+    cu = lambda o: torch.tensor(o, dtype=torch.int32, device="cuda")  # noqa: E731
+    cases = [(lambda q, s, o: topk_distill_loss(q, ids[s], t6.expand(q.shape[0], 6))),
+             (lambda q, s, o: topk_distill_loss(q, big[s], t300.expand(q.shape[0], 300))),
+             (lambda q, s, o: clipped_policy_loss(q, y[s], old[s], adv[s], clip_high=99.0).loss),
+             (lambda q, s, o: preference_loss(q, y[s], cu(o), old[s]).loss)]
+    for f in cases:
+        loss, kept = f(z, slice(None), off), f(zk, on, offk)
+        (gz,), (gk,) = torch.autograd.grad(loss, z), torch.autograd.grad(kept, zk)
+        # the same rows in another place: only the order of the sum over rows differs
+        assert abs(loss.item() - kept.item()) <= 2.0**-22 * abs(kept.item())
+        # (the preference loss's row factors come from that sum)
+        assert (gz[on].float() - gk.float()).abs().max().item() <= 2.0**-7 * gk.abs().max().item()
+        assert not gz[~on].any() and gz[on].isfinite().all()
+        del gz, gk
+        with torch.no_grad():
+            assert abs(f(z, slice(None), off).item() - loss.item()) <= 2.0**-22 * abs(loss.item())
