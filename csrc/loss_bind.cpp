@@ -196,7 +196,7 @@ void set_offsets(sepx::VocabLossArgs& a, const at::Tensor& offsets, const at::Te
 
 // Returns (loss, rewards [2 * pairs], logp [T], rows [4, T]: the rows' lse as T pairs, then
 // d loss / d logp, then scratch). With `grad` (may be the logits), d logp / d logits of each
-// row is written there, negated.
+// row is written there.
 std::vector<at::Tensor> preference_fwd(const at::Tensor& z, const at::Tensor& labels, const at::Tensor& offsets,
                                        const at::Tensor& ref_logp, double beta, double eps,
                                        const c10::optional<at::Tensor>& grad) {

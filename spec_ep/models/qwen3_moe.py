@@ -27,10 +27,11 @@ import torch.nn.functional as F
 
 from ..ops.attention import causal_gqa_attention
 from ..ops.linear import dense_fwd, linear
-from ..ops.loss import lm_head_xent
+from ..ops.loss import (PolicyLoss, lm_head_distill, lm_head_policy, lm_head_token_logp,
+                        lm_head_xent)
 from ..ops.norm import add_rms_norm, rms_norm, rms_norm_res
 from ..ops.rope import qk_norm_rope
-from ..ops.router import router_topk
+from ..ops.router import router_topk, router_topk_balanced
 from ..parallel.ep import ExpertParallel, ep_moe
 from .config import MoEModelConfig
 
@@ -62,6 +63,9 @@ class Qwen3MoeLayer(nn.Module):
         self.router_logit_bias = None  # optional fp32 [E] bias added to the router logits (skew studies)
         self.routing_callback = None  # receives topk expert ids (routing capture)
         self.spec = None  # SpeculativeExperts (speculative replication, inference only)
+        self.balance = False  # training: route with the balance loss, into the two below
+        self.balance_loss = None  # this forward's loss, until the model has added it to its own
+        self.expert_counts = None  # tokens of the last forward that chose each expert, [E] int32
 
     def forward(self, x, pos=None):
         cfg = self.cfg
@@ -82,10 +86,14 @@ class Qwen3MoeLayer(nn.Module):
                                cfg.rope_theta, pos)
         a = causal_gqa_attention(q, k, v)
         x, h = add_rms_norm(x, linear(a, self.w_o), self.post_norm, cfg.rms_norm_eps)
-        logits = linear(h, self.w_router).float()
+        logits = linear(h, self.w_router)
         if self.router_logit_bias is not None:
-            logits = logits + self.router_logit_bias
-        topk_w, topk_e = router_topk(logits, cfg.top_k, cfg.norm_topk_prob, self.router_bias)
+            logits = logits.float() + self.router_logit_bias
+        if self.balance and torch.is_grad_enabled():
+            topk_w, topk_e, self.balance_loss, self.expert_counts = router_topk_balanced(
+                logits, cfg.top_k, cfg.norm_topk_prob, self.router_bias)
+        else:
+            topk_w, topk_e = router_topk(logits.float(), cfg.top_k, cfg.norm_topk_prob, self.router_bias)
         if self.routing_callback is not None:
             self.routing_callback(topk_e)
         if spec is not None:
@@ -95,12 +103,15 @@ class Qwen3MoeLayer(nn.Module):
 
 
 class Qwen3MoeForCausalLM(nn.Module):
-    """Decoder-only MoE LM; ``forward(input_ids, labels)`` returns the mean CE loss."""
+    """Decoder-only MoE LM; ``forward(input_ids, labels)`` returns the mean CE loss, ``distill``
+    and ``policy`` the losses of their names. ``set_balance_loss`` adds the routers' balance
+    loss to each."""
 
     def __init__(self, cfg: MoEModelConfig, ep: ExpertParallel, device=None, dtype=torch.bfloat16):
         super().__init__()
         device = device or ep.device
         self.cfg, self.ep = cfg, ep
+        self.balance_coef = 0.0
         self.embed = nn.Parameter(_normal((cfg.vocab_size, cfg.hidden_size), cfg.initializer_range, device, dtype))
         self.layers = nn.ModuleList([Qwen3MoeLayer(cfg, ep, device, dtype) for _ in range(cfg.num_layers)])
         self.final_norm = nn.Parameter(torch.ones(cfg.hidden_size, device=device, dtype=dtype))
@@ -120,6 +131,23 @@ class Qwen3MoeForCausalLM(nn.Module):
         for layer in self.layers:
             layer.grad_sink = sink
 
+    def set_balance_loss(self, coef: float):
+        """Add ``coef`` times the layers' mean router balance loss to every training loss
+        (0: off). Each layer then also keeps its last forward's ``expert_counts``."""
+        if not coef >= 0.0:
+            raise ValueError(f"the balance loss's coefficient must be >= 0, not {coef}")
+        self.balance_coef = float(coef)
+        for layer in self.layers:
+            layer.balance = coef > 0.0
+
+    def _with_balance(self, loss):
+        if self.balance_coef == 0.0 or not torch.is_grad_enabled():
+            return loss
+        parts = [layer.balance_loss for layer in self.layers]
+        for layer in self.layers:
+            layer.balance_loss = None  # its graph lives as long as the loss's
+        return loss + self.balance_coef * torch.stack(parts).mean()
+
     def hidden_states(self, input_ids, pos=None):
         x = F.embedding(input_ids.view(-1), self.embed)
         for layer in self.layers:
@@ -130,4 +158,24 @@ class Qwen3MoeForCausalLM(nn.Module):
         h = self.hidden_states(input_ids, pos)
         if labels is None:
             return dense_fwd(h, self.lm_head)
-        return lm_head_xent(h, self.lm_head, labels.view(-1), num_valid)
+        return self._with_balance(lm_head_xent(h, self.lm_head, labels.view(-1), num_valid))
+
+    def distill(self, input_ids, teacher_ids, teacher_logits, temperature=1.0, num_valid=None, pos=None):
+        """Distillation loss of one token stream from a teacher's top logits ``[T, K]`` per
+        token (see ``spec_ep.ops.loss.topk_distill_loss``)."""
+        h = self.hidden_states(input_ids, pos)
+        return self._with_balance(lm_head_distill(h, self.lm_head, teacher_ids, teacher_logits, temperature, num_valid))
+
+    def policy(self, input_ids, actions, old_logp, advantages, ref_logp=None, pos=None, **kw) -> PolicyLoss:
+        """Clipped policy loss of one token stream: ``actions[t]`` is the token chosen after
+        token ``t``, -1 where none was (see ``spec_ep.ops.loss.clipped_policy_loss``, whose
+        other arguments go through ``kw``)."""
+        h = self.hidden_states(input_ids, pos)
+        out = lm_head_policy(h, self.lm_head, actions.view(-1), old_logp, advantages, ref_logp, **kw)
+        return out._replace(loss=self._with_balance(out.loss))
+
+    @torch.no_grad()
+    def token_logp(self, input_ids, labels, temperature=1.0, pos=None):
+        """Log-probability of each label (0 where it is below 0): a rollout's ``old_logp``,
+        or, from a reference model, the losses' ``ref_logp``."""
+        return lm_head_token_logp(self.hidden_states(input_ids, pos), self.lm_head, labels.view(-1), temperature)

@@ -19,6 +19,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._ext import load
 from .linear import dense_dgrad, dense_fwd, dense_wgrad
@@ -162,3 +163,88 @@ def preference_loss(logits: torch.Tensor, labels: torch.Tensor, seq_offsets: tor
     """
     return PreferenceLoss(*load().preference(logits, labels.contiguous(), seq_offsets.contiguous(), _f32(ref_logp),
                                              float(beta), float(label_smoothing)))
+
+
+# ----------------------------------------------------------------------------------------
+# the same behind the LM head: ``h [T, H] @ w[V, H].T`` gives the logits, which are kept in
+# bf16 and overwritten with their gradient
+# ----------------------------------------------------------------------------------------
+class _LMHead(torch.autograd.Function):
+    """``kernel(logits, grad)`` returns ``(loss, row_scale, *aux)``: with ``row_scale [T]`` the
+    gradient that it leaves is still to be multiplied by a factor per row."""
+
+    @staticmethod
+    def forward(ctx, h, w, kernel):
+        logits = dense_fwd(h, w)
+        loss, row_scale, *aux = kernel(logits, logits)
+        ctx.save_for_backward(h, w, logits, row_scale)
+        ctx.mark_non_differentiable(*aux)
+        ctx.set_materialize_grads(False)
+        return (loss, *aux)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, up, *_):
+        if up is None:
+            return None, None, None
+        h, w, dlogits, row_scale = ctx.saved_tensors
+        if row_scale is None:
+            return dense_dgrad(dlogits, w) * up.to(h.dtype), dense_wgrad(dlogits, h) * up.to(w.dtype), None
+        # the rows' factors go to the small side of each product: onto dh, and onto h, where
+        # they cost one more rounding to bf16 (2^-9 of each term of a sum over tokens)
+        s = (row_scale * up)[:, None]
+        return (dense_dgrad(dlogits, w) * s).to(h.dtype), dense_wgrad(dlogits, (h * s).to(h.dtype)), None
+
+
+def _lm_head(h, w, kernel):
+    if torch.is_grad_enabled() and (h.requires_grad or w.requires_grad):
+        return _LMHead.apply(h, w, kernel)
+    loss, _, *aux = kernel(dense_fwd(h, w), None)
+    return (loss, *aux)
+
+
+def lm_head_distill(h: torch.Tensor, w: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+                    temperature: float = 1.0, num_valid: int | None = None) -> torch.Tensor:
+    """``topk_distill_loss`` of the logits ``h @ w.T``, with gradients for ``h`` and ``w``."""
+    ids, t, n = teacher_ids.contiguous(), _f32(teacher_logits), _valid(num_valid)
+
+    def kernel(logits, grad):
+        return load().distill_loss(logits, ids, t, float(temperature), n, grad, None), None
+
+    return _lm_head(h, w, kernel)[0]
+
+
+def lm_head_policy(h: torch.Tensor, w: torch.Tensor, actions: torch.Tensor, old_logp: torch.Tensor,
+                   advantages: torch.Tensor, ref_logp: torch.Tensor | None = None, clip_low: float = 0.2,
+                   clip_high: float = 0.2, kl_coef: float = 0.0, temperature: float = 1.0,
+                   num_valid: int | None = None) -> PolicyLoss:
+    """``clipped_policy_loss`` of the logits ``h @ w.T``, with gradients for ``h`` and ``w``."""
+    a, old, adv, n = actions.contiguous(), _f32(old_logp), _f32(advantages), _valid(num_valid)
+    ref = None if ref_logp is None else _f32(ref_logp)
+
+    def kernel(logits, grad):
+        loss, logp, kl = load().policy_loss(logits, a, old, adv, ref, float(clip_low), float(clip_high),
+                                            float(kl_coef), float(temperature), n, grad, None)
+        return loss, None, logp, kl
+
+    return PolicyLoss(*_lm_head(h, w, kernel))
+
+
+def lm_head_preference(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, seq_offsets: torch.Tensor,
+                       ref_logp: torch.Tensor, beta: float = 0.1, label_smoothing: float = 0.0) -> PreferenceLoss:
+    """``preference_loss`` of the logits ``h @ w.T``, with gradients for ``h`` and ``w``. The
+    logits are read once: their gradient per unit of each row's factor is written in the
+    forward, and the factors, known after the whole pair, join in the backward."""
+    y, off, ref = labels.contiguous(), seq_offsets.contiguous(), _f32(ref_logp)
+
+    def kernel(logits, grad):
+        loss, rewards, logp, rows = load().preference_fwd(logits, y, off, ref, float(beta), float(label_smoothing),
+                                                          grad)
+        return loss, rows[2], rewards, logp
+
+    return PreferenceLoss(*_lm_head(h, w, kernel))
+
+
+def lm_head_token_logp(h: torch.Tensor, w: torch.Tensor, labels: torch.Tensor, temperature: float = 1.0):
+    """``token_logp`` of the logits ``h @ w.T``."""
+    return token_logp(dense_fwd(h.detach(), w.detach()), labels, temperature)

@@ -172,6 +172,8 @@ def main(argv=None):
     ap.add_argument("--micro-batch", type=int, default=1)
     ap.add_argument("--steps", type=int, default=10)
     ap.add_argument("--lr", type=float, default=1e-4)
+    ap.add_argument("--balance-coef", type=float, default=0.0,
+                    help="coefficient of the routers' load-balance loss (0 = off)")
     ap.add_argument("--expert-state", choices=["auto", "fp32", "8bit"], default="auto")
     ap.add_argument("--token-file", default=None)
     ap.add_argument("--token-dtype", default="uint32")
@@ -208,6 +210,7 @@ def main(argv=None):
                                       int(0.9 * torch.cuda.get_device_properties(dev).total_memory), act)
     torch.manual_seed(args.seed)  # replicated dense init
     model = Qwen3MoeForCausalLM(cfg, ep, device=dev)
+    model.set_balance_loss(args.balance_coef)
     trainer = Trainer(model, lr=args.lr, expert_state=prec)
     start = 0
     if args.resume:

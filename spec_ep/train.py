@@ -67,19 +67,19 @@ class Trainer:
         if self.buckets is not None:
             self.buckets.finish()
 
-    def _forward(self, input_ids, labels, num_valid):
-        """The loss, with the MoE layers' receive buffers sized by row budgets (no host
+    def _forward(self, loss_fn):
+        """``loss_fn()``, with the MoE layers' receive buffers sized by row budgets (no host
         wait between layers). If some layer's rows outgrew its budget on any rank, the
         forward is discarded (nothing was updated yet) and run again with the grown
         budgets; the first step learns the budgets with exact sizes."""
         ep = getattr(self.model, "ep", None)
         if ep is None or not hasattr(ep, "run_pass"):
-            return self.model(input_ids, labels, num_valid)
+            return loss_fn()
         calls = [0]
 
         def fwd():
             calls[0] += 1
-            return self.model(input_ids, labels, num_valid)
+            return loss_fn()
 
         loss = ep.run_pass(fwd)
         self.budget_retries += calls[0] - 1
@@ -87,9 +87,15 @@ class Trainer:
 
     def train_step(self, input_ids, labels, num_valid=None):
         """One optimizer step on a device-resident batch; returns the (device) loss."""
+        return self.step(lambda: self.model(input_ids, labels, num_valid))
+
+    def step(self, loss_fn):
+        """One optimizer step on ``loss_fn()``, a scalar loss of the model (one forward of
+        it, which may run again when row budgets were outgrown): for instance
+        ``trainer.step(lambda: model.policy(ids, actions, old, adv).loss)``."""
         if self.buckets is not None:
             self.buckets.begin()
-        loss = self._forward(input_ids, labels, num_valid)
+        loss = self._forward(loss_fn)
         loss.backward()
         self.expert_updater.flush()
         self._sync_dense_grads()
