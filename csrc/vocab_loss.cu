@@ -835,7 +835,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
     // A row's sum is complete some 2500 cycles before its factor is back from the other
     // warps and blocks: meanwhile the sum of the next row begins, over the pieces that are
     // there already.
-    constexpr int kAhead = 3;
+    constexpr int kAhead = 3;  // the first piece and a pair
     const int tid = threadIdx.x;
     uint4 none;  // a vector of -infinity
     {
@@ -846,6 +846,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
     }
     const C2 c2 = {a.c2, a.c2_lo};
     const F2 cc = f2(a.c2, a.c2), cl = f2(a.c2_lo, a.c2_lo);
+    auto piece_at = [&](int sl) { return reinterpret_cast<const uint4*>(ring + (size_t)sl * kPieceBytes) + tid; };
     int slot = 0, turn = 0, grad_slot = 0, e = 0, lap = 0, x = 0;
     // the row that is summed: done of np pieces
     int t = cluster, np = 0, done = 0, part_n = 0;
@@ -889,15 +890,81 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
         // may grow to 2^40 before the reference is moved, which costs fp32 nothing, so the
         // usual vector takes no maximum.
         const int stop = tg >= 0 ? min(np, done + kAhead) : np;
-        for (; done < stop; ++done) {
+        auto there = [&](int sl, int tn) {  // a row's gradient is owed: do not wait
+          return __all_sync(0xffffffffu, mbar_test_wait(&sh.full[sl], (uint32_t)tn)) != 0;
+        };
+        auto add_vec = [&](const uint4& raw, F2 (&acc)[2]) {
+          float o[N];
+          Elem<T>::unpack(raw, o);
+#pragma unroll
+          for (int i = 0; i < N; i += 2) {
+            const F2 z2 = f2(o[i], o[i + 1]);
+            acc[(i >> 1) & 1] = add2(acc[(i >> 1) & 1], ex2_2(fma2(z2, cl, fma2(z2, cc, nR2))));
+          }
+        };
+        auto total = [&](F2 (&acc)[2]) {
+          float ax, ay;
+          split(add2(acc[0], acc[1]), ax, ay);
+          return sum + (ax + ay);
+        };
+        auto add_carefully = [&](const uint4* piece, int n, bool first) {
+          const float2 r = careful_sum<T>(piece, n, Cfg::Lanes, c2, first ? -INFINITY : ref, sum);
+          ref = r.x;
+          sum = r.y;
+          const float R = reference(ref, c2);
+          nR2 = f2(R, R);
+        };
+        auto next_slot = [&] {
+          if (!a.grad) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.empty[slot]);
+          }
+          if (++slot == slots) {
+            slot = 0;
+            turn ^= 1;
+          }
+        };
+        while (done < stop) {
           if (tg >= 0) {
-            if (!__all_sync(0xffffffffu, mbar_test_wait(&sh.full[slot], (uint32_t)turn))) break;
+            if (!there(slot, turn)) break;
           } else if (!wait(&sh.full[slot], turn)) {
             goto out;
           }
           const int end = part_n - done * kPieceVecs;                // vectors left
-          const int left = (end - tid + Cfg::Lanes - 1) / Cfg::Lanes;  // of them this thread's (or < 1)
-          const uint4* piece = reinterpret_cast<const uint4*>(ring + (size_t)slot * kPieceBytes) + tid;
+          const uint4* piece = piece_at(slot);
+          // After the first piece two whole ones at a time, for more arithmetic between the
+          // waits. Where the sum is split depends on the place in the row alone, never on
+          // what has arrived: the same bits on every run.
+          if (done > 0 && end >= 2 * kPieceVecs) {
+            const int slot1 = slot + 1 == slots ? 0 : slot + 1, turn1 = slot + 1 == slots ? turn ^ 1 : turn;
+            if (tg >= 0) {
+              if (!there(slot1, turn1)) break;
+            } else if (!wait(&sh.full[slot1], turn1)) {
+              goto out;
+            }
+            const uint4* piece1 = piece_at(slot1);
+            uint4 raw[2 * Cfg::VPT];
+#pragma unroll
+            for (int v = 0; v < Cfg::VPT; ++v) {
+              raw[v] = piece[v * Cfg::Lanes];
+              raw[Cfg::VPT + v] = piece1[v * Cfg::Lanes];
+            }
+            F2 acc[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+#pragma unroll
+            for (int v = 0; v < 2 * Cfg::VPT; ++v) add_vec(raw[v], acc);
+            const float s1 = total(acc);
+            if (s1 <= 1.0995e12f) {
+              sum = s1;
+            } else {  // NaN too
+              add_carefully(piece, Cfg::VPT, false);
+              add_carefully(piece1, Cfg::VPT, false);
+            }
+            done += 2;
+            next_slot();
+            next_slot();
+            continue;
+          }
+          const int left = (end - tid + Cfg::Lanes - 1) / Cfg::Lanes;  // this thread's vectors (or < 1)
           uint4 raw[Cfg::VPT];
           if (end >= kPieceVecs) {
 #pragma unroll
@@ -916,34 +983,13 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
 #pragma unroll
           for (int v = 0; v < Cfg::VPT; ++v) {
             if (v > 0 && end <= v * Cfg::Lanes) break;  // nothing left for any thread
-            float o[N];
-            Elem<T>::unpack(raw[v], o);
-#pragma unroll
-            for (int i = 0; i < N; i += 2) {
-              const F2 z2 = f2(o[i], o[i + 1]);
-              acc[(i >> 1) & 1] = add2(acc[(i >> 1) & 1], ex2_2(fma2(z2, cl, fma2(z2, cc, nR2))));
-            }
+            add_vec(raw[v], acc);
           }
-          float ax, ay;
-          split(add2(acc[0], acc[1]), ax, ay);
-          const float s1 = sum + (ax + ay);
-          if (s1 <= 1.0995e12f) {
-            sum = s1;
-          } else if (left > 0) {  // NaN too
-            const float2 r = careful_sum<T>(piece, min(left, Cfg::VPT), Cfg::Lanes, c2, done == 0 ? -INFINITY : ref, sum);
-            ref = r.x;
-            sum = r.y;
-            const float R = reference(ref, c2);
-            nR2 = f2(R, R);
-          }
-          if (!a.grad) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.empty[slot]);
-          }
-          if (++slot == slots) {
-            slot = 0;
-            turn ^= 1;
-          }
+          const float s1 = total(acc);
+          if (s1 <= 1.0995e12f) sum = s1;
+          else if (left > 0) add_carefully(piece, min(left, Cfg::VPT), done == 0);  // NaN too
+          ++done;
+          next_slot();
         }
       }
       if (tg >= 0) {
@@ -960,34 +1006,57 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
         // whole vectors of this part: pieces within them take the straight path
         const int lo = z.full(0) ? 0 : 1, hi = z.full(z.nv - 1) ? z.nv : z.nv - 1;
         T* gp = g.p + z.first(j0 + tid);
-        for (int base = j0; base < j1; base += kPieceVecs, gp += kPieceVecs * N) {
-          const uint4* piece = reinterpret_cast<const uint4*>(ring + (size_t)grad_slot * kPieceBytes) + tid;
-          auto grad_vec = [&](const uint4& raw, int v) {
-            float o[N];
-            Elem<T>::unpack(raw, o);
+        auto grad_vec = [&](const uint4& raw, T* to) {
+          float o[N];
+          Elem<T>::unpack(raw, o);
 #pragma unroll
-            for (int i = 0; i < N; i += 2)
-              split(mul2(As2, ex2_2(fma2(f2(o[i], o[i + 1]), cc, nM2))), o[i], o[i + 1]);
-            *reinterpret_cast<uint4*>(gp + v * Cfg::Lanes * N) = Elem<T>::pack(o);
-          };
-          if (plain && base >= lo && base + kPieceVecs <= min(hi, j1)) {
+          for (int i = 0; i < N; i += 2)
+            split(mul2(As2, ex2_2(fma2(f2(o[i], o[i + 1]), cc, nM2))), o[i], o[i + 1]);
+          *reinterpret_cast<uint4*>(to) = Elem<T>::pack(o);
+        };
+        auto free_slot = [&] {
+          if (lane == 0) mbar_arrive(&sh.empty[grad_slot]);
+          if (++grad_slot == slots) grad_slot = 0;
+        };
+        const int inner = plain ? min(hi, j1) : 0;
+        for (int base = j0; base < j1;) {
+          const uint4* piece = piece_at(grad_slot);
+          if (base >= lo && base + 2 * kPieceVecs <= inner) {
+            const uint4* piece1 = piece_at(grad_slot + 1 == slots ? 0 : grad_slot + 1);
+            uint4 raw[2 * Cfg::VPT];
+#pragma unroll
+            for (int v = 0; v < Cfg::VPT; ++v) {
+              raw[v] = piece[v * Cfg::Lanes];
+              raw[Cfg::VPT + v] = piece1[v * Cfg::Lanes];
+            }
+#pragma unroll
+            for (int v = 0; v < 2 * Cfg::VPT; ++v) grad_vec(raw[v], gp + v * Cfg::Lanes * N);
+            __syncwarp();
+            free_slot();
+            free_slot();
+            base += 2 * kPieceVecs;
+            gp += 2 * kPieceVecs * N;
+            continue;
+          }
+          if (base >= lo && base + kPieceVecs <= inner) {
             uint4 raw[Cfg::VPT];
 #pragma unroll
             for (int v = 0; v < Cfg::VPT; ++v) raw[v] = piece[v * Cfg::Lanes];
 #pragma unroll
-            for (int v = 0; v < Cfg::VPT; ++v) grad_vec(raw[v], v);
+            for (int v = 0; v < Cfg::VPT; ++v) grad_vec(raw[v], gp + v * Cfg::Lanes * N);
           } else {  // a row's end in this piece, another phase, or a far reference
 #pragma unroll 1
             for (int v = 0; v < Cfg::VPT; ++v) {
               const int j = base + tid + v * Cfg::Lanes;
               if (j >= j1) break;
-              if (plain && j >= lo && j < hi) grad_vec(piece[v * Cfg::Lanes], v);
+              if (plain && j >= lo && j < hi) grad_vec(piece[v * Cfg::Lanes], gp + v * Cfg::Lanes * N);
               else careful_store<T>(piece + v * Cfg::Lanes, g.p, a.V, z.first(j), c2, m, As);
             }
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.empty[grad_slot]);
-          if (++grad_slot == slots) grad_slot = 0;
+          free_slot();
+          base += kPieceVecs;
+          gp += kPieceVecs * N;
         }
         if constexpr (OP != kOpDistill) {  // the token's element, from the thread that wrote its vector
           const Token token = sh.token[eg];

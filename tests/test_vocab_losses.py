@@ -349,6 +349,21 @@ def test_same_bits_on_every_run_and_on_another_stream(i):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [1000, 8000, 40001, 151936])
+@pytest.mark.parametrize("i", [0, 1, 2])
+def test_same_bits_over_many_long_rows(i, V):
+    """Several rows per block, so that a row's sum begins while another's gradient is owed:
+    where the sums are split must not depend on what has arrived."""
+    z, _ = _logits(1300 if V < 100000 else 500, V, "bf16", False, 4)
+    loss = _three(z, i)
+    (g,) = torch.autograd.grad(loss, z)
+    for _ in range(4):
+        l2 = _three(z, i)
+        (g2,) = torch.autograd.grad(l2, z)
+        assert torch.equal(loss, l2) and torch.equal(g, g2)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("i", [0, 1, 2])
 def test_two_captured_graphs_replay_with_new_inputs(i):
     """Forward and backward captured twice, replayed in turn over changed logits."""
