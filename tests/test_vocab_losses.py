@@ -604,15 +604,20 @@ def test_many_rows_out_of_the_loss(V, pattern):
     t6, t300 = torch.linspace(1, 0, 6, device="cuda"), torch.linspace(2, 0, 300, device="cuda")
     off, offk = ([0, T // 2, T], [0, int(on[:T // 2].sum()), n])
     cu = lambda o: torch.tensor(o, dtype=torch.int32, device="cuda")  # noqa: E731
-    cases = [(lambda q, s, o: topk_distill_loss(q, ids[s], t6.expand(q.shape[0], 6))),
-             (lambda q, s, o: topk_distill_loss(q, big[s], t300.expand(q.shape[0], 300))),
-             (lambda q, s, o: clipped_policy_loss(q, y[s], old[s], adv[s], clip_high=99.0).loss),
-             (lambda q, s, o: preference_loss(q, y[s], cu(o), old[s]).loss)]
-    for f in cases:
+    # d loss / d (a common error of all log-probabilities): the weights sum to 1; r A with every
+    # A > 0; beta / 2 per row of either sequence
+    cases = [(lambda q, s, o: topk_distill_loss(q, ids[s], t6.expand(q.shape[0], 6)), lambda v: 1.0),
+             (lambda q, s, o: topk_distill_loss(q, big[s], t300.expand(q.shape[0], 300)), lambda v: 1.0),
+             (lambda q, s, o: clipped_policy_loss(q, y[s], old[s], adv[s], clip_high=99.0).loss, abs),
+             (lambda q, s, o: preference_loss(q, y[s], cu(o), old[s]).loss, lambda v: 0.1 * n)]
+    for f, slope in cases:
         loss, kept = f(z, slice(None), off), f(zk, on, offk)
         (gz,), (gk,) = torch.autograd.grad(loss, z), torch.autograd.grad(kept, zk)
-        # the same rows in another place: only the order of the sum over rows differs
-        assert abs(loss.item() - kept.item()) <= 2.0**-22 * abs(kept.item())
+        # The same rows in another place: the sum over rows has another order (64 bits), and
+        # with an odd vocabulary a row begins elsewhere in its 16 bytes, so the row's own
+        # fp32 sum is grouped differently: both are within _lse_tol of the exact one.
+        tol = 2.0**-22 * abs(kept.item()) + (V % 8 > 0) * 2 * _lse_tol(V) * slope(kept.item())
+        assert abs(loss.item() - kept.item()) <= tol
         # (the preference loss's row factors come from that sum)
         assert (gz[on].float() - gk.float()).abs().max().item() <= 2.0**-7 * gk.abs().max().item()
         assert not gz[~on].any() and gz[on].isfinite().all()
