@@ -1279,35 +1279,69 @@ __global__ void __launch_bounds__(256) preference_pairs_kernel(const PreferenceA
   if (threadIdx.x == 0) *a.loss = (float)(v / a.pairs);
 }
 
-// dz = up * row_coef * (onehot - softmax) from the saved log-sum-exp: one read, one write.
+// dz = up * row_coef * (onehot - softmax) from the saved reference and sum: one read, one
+// write. Rows go from the last to the first: the forward has just read the last ones, and
+// what of them is still in L2 is not fetched again (the gradient is written around it).
+constexpr int kGradThreads = 256, kGradVecs = 4, kGradChunk = 2 * kGradThreads * kGradVecs;
 template <typename T>
-__global__ void __launch_bounds__(256) preference_grad_kernel(const VocabLossArgs a, const float* __restrict__ row_coef,
-                                                              int chunks, int chunk) {
+__global__ void __launch_bounds__(kGradThreads) preference_grad_kernel(const VocabLossArgs a,
+                                                                       const float* __restrict__ row_coef, int chunks) {
   constexpr int N = Elem<T>::N;
-  const int t = blockIdx.x / chunks, c = blockIdx.x % chunks;
+  const int t = a.T - 1 - (int)(blockIdx.x / (unsigned)chunks), c = (int)(blockIdx.x % (unsigned)chunks);
+  const int tid = threadIdx.x;
   const RowVec<T> z(const_cast<T*>(reinterpret_cast<const T*>(a.z)) + (int64_t)t * a.z_stride, a.V);
   const RowVec<T> g(reinterpret_cast<T*>(a.grad) + (int64_t)t * a.grad_stride, a.V);
-  const int j0 = c * chunk, j1 = min(j0 + chunk, z.nv);
+  const int j0 = c * kGradChunk, j1 = min(j0 + kGradChunk, z.nv);
   const int64_t label = load_id(a.labels, t, a.ids64);
   const float coef = row_coef[t];
+  const float2 l = reinterpret_cast<const float2*>(a.lse)[t];
   // rows outside the loss are not read: their logits may hold anything
   const bool on = label >= 0 && t >= a.offsets[0] && t < a.offsets[a.num_seq];
-  const float A = on ? -coef * *a.up : 0.f;
-  const float2 l = reinterpret_cast<const float2*>(a.lse)[t];  // the row's maximum and sum
-  const Expo x(C2{a.c2, a.c2_lo}, l.x);
-  const float As = A / l.y;
-  for (int j = j0 + threadIdx.x; j < j1; j += blockDim.x) {
-    float o[N];
-    if (on) {
-      Elem<T>::unpack(z.load(j), o);
-      const int64_t e0 = z.first(j);
-#pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = fmaf(As, x(o[i]), e0 + i == label ? -A : 0.f);
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = 0.f;
+  // whole vectors at the same phase take the straight path
+  const bool same = g.a == z.a;
+  const int lo = z.full(0) ? 0 : 1, hi = z.full(z.nv - 1) ? z.nv : z.nv - 1;
+  if (!on) {
+    const float o[N] = {};
+    for (int j = j0 + tid; j < j1; j += kGradThreads) {
+      if (same && j >= lo && j < hi) __stcs(reinterpret_cast<uint4*>(g.p + z.first(j)), make_uint4(0, 0, 0, 0));
+      else g.store(z.first(j), o);
     }
-    g.store(z.first(j), o);
+    return;
+  }
+  const float A = -coef * *a.up, As = A / l.y;
+  const C2 c2 = {a.c2, a.c2_lo};
+  const Expo x(c2, l.x);
+  const bool plain = same && !x.far;
+  const F2 cc = f2(a.c2, a.c2), nM2 = f2(-x.M2, -x.M2), As2 = f2(As, As);
+  for (int base = j0; base < j1; base += kGradThreads * kGradVecs) {
+    uint4 raw[kGradVecs];
+#pragma unroll
+    for (int v = 0; v < kGradVecs; ++v) {
+      const int j = base + v * kGradThreads + tid;
+      if (j >= lo && j < min(hi, j1)) raw[v] = __ldg(reinterpret_cast<const uint4*>(z.p + z.first(j)));
+    }
+#pragma unroll
+    for (int v = 0; v < kGradVecs; ++v) {
+      const int j = base + v * kGradThreads + tid;
+      if (j >= j1) break;
+      if (plain && j >= lo && j < hi) {
+        float o[N];
+        Elem<T>::unpack(raw[v], o);
+#pragma unroll
+        for (int i = 0; i < N; i += 2)
+          split(mul2(As2, ex2_2(fma2(f2(o[i], o[i + 1]), cc, nM2))), o[i], o[i + 1]);
+        __stcs(reinterpret_cast<uint4*>(g.p + z.first(j)), Elem<T>::pack(o));
+      } else {
+        const uint4 r = z.load(j);
+        careful_store<T>(&r, g.p, a.V, z.first(j), c2, l.x, As);
+      }
+    }
+  }
+  // the label's element, from the thread that wrote its vector
+  if (label < a.V) {
+    const int own = (int)((label + z.a) / N) - j0;
+    if (own >= 0 && own < j1 - j0 && own % kGradThreads == tid)
+      g.p[label] = Elem<T>::t(As * x(Elem<T>::f(z.p[label])) - A);
   }
 }
 
@@ -1477,13 +1511,14 @@ void preference_grad(const VocabLossArgs& a, const float* row_coef, cudaStream_t
   if (a.T <= 0) return;
   const int n = a.dtype == kVocabF32 ? 4 : 8;
   const int nv = (int)(((int64_t)a.V + 2 * n - 2) / n);  // vectors of a row at its worst phase
-  const int chunk = 2048, chunks = (nv + chunk - 1) / chunk;
+  const int chunks = (nv + kGradChunk - 1) / kGradChunk;
   const int64_t blocks = (int64_t)a.T * chunks;
   if (blocks > 0x7fffffff) throw std::runtime_error("preference_grad: too many rows");
   if (a.dtype == kVocabBf16)
-    preference_grad_kernel<__nv_bfloat16><<<(int)blocks, 256, 0, st>>>(a, row_coef, chunks, chunk);
-  else if (a.dtype == kVocabF16) preference_grad_kernel<__half><<<(int)blocks, 256, 0, st>>>(a, row_coef, chunks, chunk);
-  else preference_grad_kernel<float><<<(int)blocks, 256, 0, st>>>(a, row_coef, chunks, chunk);
+    preference_grad_kernel<__nv_bfloat16><<<(int)blocks, kGradThreads, 0, st>>>(a, row_coef, chunks);
+  else if (a.dtype == kVocabF16)
+    preference_grad_kernel<__half><<<(int)blocks, kGradThreads, 0, st>>>(a, row_coef, chunks);
+  else preference_grad_kernel<float><<<(int)blocks, kGradThreads, 0, st>>>(a, row_coef, chunks);
   check_launch("preference_grad");
 }
 
