@@ -8,6 +8,12 @@
 // tokens; blocks write partial sums and a second kernel adds them in a fixed order, so the
 // loss has the same bits on every run. The backward recomputes p from the logits instead of
 // reading it back: T x E fp32 probabilities are never stored.
+//
+// What bounds it: arithmetic, not memory. 65537 tokens x 256 experts in fp32 would take 10 us
+// (forward) and 21 us (backward) at 6.55 TB/s; measured 48 us with the sum kernel and 32 us.
+// The forward executes 480 instructions per token and warp (sorting, 8 choices, softmax),
+// the integer pipe 63% busy; the backward 295. Choosing by scanning all scores for every
+// choice took 80 us, with the experts' indices carried beside the keys 72 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -23,7 +29,7 @@
 namespace sepx {
 namespace {
 
-constexpr int kWarps = 8, kFwdWarps = 16;
+constexpr int kWarps = 8, kFwdWarps = 32;
 
 void check_launch(const char* what) {
   note_launch();
@@ -227,7 +233,7 @@ __device__ __forceinline__ int choose(int E, int k, int lane, const float (&scor
 template <typename T, int EPL, int VEC>
 __global__ void __launch_bounds__(kFwdWarps * 32) router_balance_fwd_kernel(const RouterBalanceArgs a) {
   __shared__ int s_cnt[EPL * 32];
-  __shared__ float s_p[kFwdWarps][EPL * 32];
+  __shared__ float s_p[kFwdWarps / 2][EPL * 32];
   __shared__ int s_n;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int e = threadIdx.x; e < EPL * 32; e += blockDim.x) s_cnt[e] = 0;
@@ -278,14 +284,20 @@ __global__ void __launch_bounds__(kFwdWarps * 32) router_balance_fwd_kernel(cons
       if (on) atomicAdd(&s_cnt[my_e], 1);
     }
   }
+  // the warps' sums in a fixed order: the upper half onto the lower one, then down the rows
+  if (warp >= kFwdWarps / 2)
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) s_p[warp][expert_of<VEC>(i, lane)] = acc[i];
+    for (int i = 0; i < EPL; ++i) s_p[warp - kFwdWarps / 2][expert_of<VEC>(i, lane)] = acc[i];
   if (lane == 0 && n) atomicAdd(&s_n, n);
+  __syncthreads();
+  if (warp < kFwdWarps / 2)
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) s_p[warp][expert_of<VEC>(i, lane)] += acc[i];
   __syncthreads();
   for (int e = threadIdx.x; e < a.E; e += blockDim.x) {
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < kFwdWarps; ++w) s += s_p[w][e];
+    for (int w = 0; w < kFwdWarps / 2; ++w) s += s_p[w][e];
     a.part_p[(int64_t)blockIdx.x * a.E + e] = s;
     a.part_c[(int64_t)blockIdx.x * a.E + e] = s_cnt[e];
   }
@@ -450,7 +462,7 @@ void check_args(const RouterBalanceArgs& a) {
 
 }  // namespace
 
-int router_balance_blocks(int T, int num_sms) { return std::max(1, std::min((T + kFwdWarps - 1) / kFwdWarps, num_sms * 2)); }
+int router_balance_blocks(int T, int num_sms) { return std::max(1, std::min((T + kFwdWarps - 1) / kFwdWarps, num_sms)); }
 
 void router_balance_fwd(const RouterBalanceArgs& a, cudaStream_t st) {
   check_args(a);
