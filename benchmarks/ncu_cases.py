@@ -22,6 +22,10 @@ most, so a ``--set full`` capture of one launch ends in seconds:
             -> 2048)
   swiglu_bwd  CTA-pair down-projection dgrad + SwiGLU backward epilogue, 16 experts x 2048
             rows (the EP = 8 layout)
+  losses    distillation (64 teacher entries) and preference loss, each with its gradient,
+            1024 rows of a 151,936 vocabulary (bf16 logits)
+  router_balance  routing with the balance loss, forward and backward, 65,537 tokens over
+            256 experts (fp32 logits, top-8)
 
     python benchmarks/ncu_cases.py --case gemm
     ncu --set full --clock-control none -k regex:grouped_gemm -s 2 -c 1 -o out python benchmarks/ncu_cases.py --case gemm
@@ -38,7 +42,8 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--case", required=True, choices=["gemm", "wgrad", "dispatch", "adamw", "wgrad_adamw8", "attn_fwd", "attn_fwd2",
-                                                       "attn_bwd", "layer_ops", "dense", "swiglu_bwd"])
+                                                       "attn_bwd", "layer_ops", "dense", "swiglu_bwd", "losses",
+                                                       "router_balance"])
     ap.add_argument("--reps", type=int, default=4)
     args = ap.parse_args()
     from spec_ep.ops import grouped_gemm as gg
@@ -81,6 +86,27 @@ def main():
                 attention_fwd(q, k, v, two_tile=args.case == "attn_fwd2")
             else:
                 attention_bwd(q, k, v, o, lse, do)
+    elif args.case == "losses":
+        from spec_ep.ops.loss import preference_loss, topk_distill_loss
+
+        T, V, K = 1024, 151936, 64
+        z = (torch.randn(T, V, device=dev) * 2).bfloat16().requires_grad_()
+        ids = torch.randint(0, V, (T, K), device=dev)
+        t = torch.randn(T, K, device=dev) * 2.5
+        y = torch.randint(0, V, (T,), device=dev)
+        off = torch.tensor([0, T // 2, T], device=dev, dtype=torch.int32)
+        ref = torch.full((T,), -13.0, device=dev)
+        for _ in range(args.reps):
+            torch.autograd.grad(topk_distill_loss(z, ids, t, num_valid=T), z)
+            torch.autograd.grad(preference_loss(z, y, off, ref).loss, z)
+    elif args.case == "router_balance":
+        from spec_ep.ops.router import router_topk_balanced
+
+        x = torch.randn(65537, 256, device=dev).bfloat16().float().requires_grad_()
+        dw = torch.randn(65537, 8, device=dev)
+        for _ in range(args.reps):
+            w, _, loss, _ = router_topk_balanced(x, 8)
+            torch.autograd.grad([w, loss], x, [dw, torch.ones_like(loss)])
     elif args.case == "layer_ops":
         from spec_ep.ops._ext import load
 
