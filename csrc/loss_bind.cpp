@@ -70,9 +70,10 @@ sepx::VocabLossArgs vocab_args(const at::Tensor& z, const c10::optional<at::Tens
   if (grad.has_value()) {
     TORCH_CHECK(grad->device() == z.device() && grad->scalar_type() == z.scalar_type() && grad->sizes() == z.sizes(),
                 "the gradient buffer must be like the logits");
-    TORCH_CHECK(grad->is_contiguous(), "the gradient buffer must be contiguous");
+    TORCH_CHECK((grad->stride(1) == 1 || grad->size(1) == 1) && (grad->stride(0) >= grad->size(1) || grad->size(0) < 2),
+                "the gradient buffer must have unit stride along the vocabulary and rows apart");
     a.grad = grad->data_ptr();
-    a.grad_stride = grad->size(1);
+    a.grad_stride = grad->stride(0);
   }
   return a;
 }
@@ -95,6 +96,22 @@ at::Tensor set_rows(sepx::VocabLossArgs& a, int op, int64_t num_valid, const at:
     sepx::vocab_count_rows(a, op, count.data_ptr<int>(), cs());
   }
   return count;
+}
+
+// Gradient of the logits, with rows at the same places in their 16 bytes as the logits' rows,
+// so that both move in whole vectors: the logits' row stride (where it costs little memory)
+// and the phase of their first row. Contiguous where the logits are.
+bool shares_stride(const at::Tensor& z) {
+  return z.dim() == 2 && z.stride(0) >= z.size(1) && z.stride(0) <= z.size(1) + z.size(1) / 64 + 64;
+}
+at::Tensor gradient_storage(const at::Tensor& z) {
+  TORCH_CHECK(z.dim() == 2, "logits must be [T, V]");
+  return at::empty({z.size(0) * (shares_stride(z) ? z.stride(0) : z.size(1)) + 16 / z.element_size()}, z.options());
+}
+at::Tensor gradient_view(const at::Tensor& flat, const at::Tensor& z) {
+  const int64_t phase = (int64_t)(reinterpret_cast<uintptr_t>(z.data_ptr()) % 16) / z.element_size();
+  return flat.as_strided({z.size(0), z.size(1)}, {shares_stride(z) ? z.stride(0) : z.size(1), 1},
+                         flat.storage_offset() + phase);
 }
 
 // Scratch of a call: records, partial sums and a ticket in one allocation.
@@ -242,7 +259,7 @@ std::vector<at::Tensor> preference_fwd(const at::Tensor& z, const at::Tensor& la
 // d (up * loss) / d logits from the forward's rows.
 at::Tensor preference_grad(const at::Tensor& z, const at::Tensor& labels, const at::Tensor& offsets,
                            const at::Tensor& rows, const at::Tensor& up) {
-  at::Tensor grad = at::empty(z.sizes(), z.options());
+  const at::Tensor grad = gradient_view(gradient_storage(z), z);
   auto a = vocab_args(z, grad, 1.0);
   req_rows(labels, z, "labels");
   TORCH_CHECK(rows.device() == z.device() && rows.scalar_type() == at::kFloat && rows.is_contiguous() &&
@@ -260,7 +277,7 @@ at::Tensor preference_grad(const at::Tensor& z, const at::Tensor& labels, const 
 }
 
 // grad *= up in place (nothing is read where up is 1).
-void scale_grad(at::Tensor& grad, const at::Tensor& up) {
+void scale_grad(const at::Tensor& grad, const at::Tensor& up) {
   TORCH_CHECK(grad.is_contiguous(), "grad must be contiguous");
   TORCH_CHECK(up.device() == grad.device() && up.numel() == 1 && up.scalar_type() == at::kFloat,
               "the gradient of the loss must be one fp32 on the same device");
@@ -381,22 +398,29 @@ at::Tensor once(AutogradContext* ctx, const at::Tensor& g) {
 // once, scaled in place (not touched where the upstream gradient is 1). A second backward
 // through the same graph, and fp16 logits, whose unscaled gradient could leave the type's
 // range, compute it from the logits.
-at::Tensor gradient_buffer(const at::Tensor& z) { return at::empty(z.sizes(), z.options()); }
 bool formed_in_forward(const at::Tensor& z) { return z.scalar_type() != at::kHalf; }
+// Keeps a buffer for the gradient and returns its view.
+at::Tensor keep_gradient(AutogradContext* ctx, const at::Tensor& z) {
+  const at::Tensor flat = gradient_storage(z), g = gradient_view(flat, z);
+  ctx->saved_data["grad"] = flat;
+  ctx->saved_data["at"] = std::vector<int64_t>{g.size(0), g.size(1), g.stride(0), g.storage_offset()};
+  return g;
+}
 at::Tensor take_formed(AutogradContext* ctx, const at::Tensor& up) {
   auto& kept = ctx->saved_data["grad"];
   if (!kept.isTensor()) return {};
-  at::Tensor g = kept.toTensor();
+  at::Tensor flat = kept.toTensor();
   kept = c10::IValue();
-  scale_grad(g, up);
-  return g;
+  scale_grad(flat, up);  // with what lies between the rows, which nothing reads
+  const auto at = ctx->saved_data["at"].toIntVector();
+  return flat.as_strided({at[0], at[1]}, {at[2], 1}, at[3]);
 }
 
 struct DistillFn : torch::autograd::Function<DistillFn> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& z, const at::Tensor& ids, const at::Tensor& teacher,
                             double tau, int64_t num_valid) {
     c10::optional<at::Tensor> grad;
-    if (formed_in_forward(z)) ctx->saved_data["grad"] = *(grad = gradient_buffer(z));
+    if (formed_in_forward(z)) grad = keep_gradient(ctx, z);
     at::Tensor loss = distill_loss(z, ids, teacher, tau, num_valid, grad, c10::nullopt);
     ctx->save_for_backward({z, ids, teacher});
     ctx->saved_data["tau"] = tau;
@@ -407,7 +431,7 @@ struct DistillFn : torch::autograd::Function<DistillFn> {
     at::Tensor g = take_formed(ctx, up[0]);
     if (!g.defined()) {
       const auto s = ctx->get_saved_variables();
-      g = gradient_buffer(s[0]);
+      g = gradient_view(gradient_storage(s[0]), s[0]);
       distill_loss(s[0], s[1], s[2], ctx->saved_data["tau"].toDouble(), ctx->saved_data["num_valid"].toInt(), g, up[0]);
     }
     return {once(ctx, g), {}, {}, {}, {}};
@@ -426,7 +450,7 @@ struct PolicyFn : torch::autograd::Function<PolicyFn> {
                                const c10::optional<at::Tensor>& ref_logp, double clip_low, double clip_high,
                                double kl_coef, double tau, int64_t num_valid) {
     c10::optional<at::Tensor> grad;
-    if (formed_in_forward(z)) ctx->saved_data["grad"] = *(grad = gradient_buffer(z));
+    if (formed_in_forward(z)) grad = keep_gradient(ctx, z);
     auto out = policy_loss(z, actions, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coef, tau, num_valid,
                            grad, c10::nullopt);
     ctx->save_for_backward({z, actions, old_logp, advantages, ref_logp.value_or(at::Tensor())});
@@ -443,7 +467,7 @@ struct PolicyFn : torch::autograd::Function<PolicyFn> {
       if (!g.defined()) {
         const auto s = ctx->get_saved_variables();
         const auto c = ctx->saved_data["cfg"].toDoubleVector();
-        g = gradient_buffer(s[0]);
+        g = gradient_view(gradient_storage(s[0]), s[0]);
         policy_loss(s[0], s[1], s[2], s[3], s[4].defined() ? c10::optional<at::Tensor>(s[4]) : c10::nullopt, c[0], c[1],
                     c[2], c[3], ctx->saved_data["num_valid"].toInt(), g, up[0]);
       }

@@ -188,12 +188,15 @@ class _LMHead(torch.autograd.Function):
         if up is None:
             return None, None, None
         h, w, dlogits, row_scale = ctx.saved_tensors
+        dh = dense_dgrad(dlogits, w) if ctx.needs_input_grad[0] else None
         if row_scale is None:
-            return dense_dgrad(dlogits, w) * up.to(h.dtype), dense_wgrad(dlogits, h) * up.to(w.dtype), None
+            dw = dense_wgrad(dlogits, h) if ctx.needs_input_grad[1] else None
+            return None if dh is None else dh * up.to(h.dtype), None if dw is None else dw * up.to(w.dtype), None
         # the rows' factors go to the small side of each product: onto dh, and onto h, where
         # they cost one more rounding to bf16 (2^-9 of each term of a sum over tokens)
         s = (row_scale * up)[:, None]
-        return (dense_dgrad(dlogits, w) * s).to(h.dtype), dense_wgrad(dlogits, (h * s).to(h.dtype)), None
+        dw = dense_wgrad(dlogits, (h * s).to(h.dtype)) if ctx.needs_input_grad[1] else None
+        return None if dh is None else (dh * s).to(h.dtype), dw, None
 
 
 def _lm_head(h, w, kernel):

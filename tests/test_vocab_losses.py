@@ -624,3 +624,38 @@ def test_many_rows_out_of_the_loss(V, pattern):
         del gz, gk
         with torch.no_grad():
             assert abs(f(z, slice(None), off).item() - loss.item()) <= 2.0**-22 * abs(loss.item())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("i", [0, 1, 2])
+def test_views_of_padded_logits(i, dtype):
+    """Logits of an odd vocabulary in rows padded to a multiple of 64, rows that start at an
+    odd place, far apart or expanded: the values of contiguous ones. Row sums are grouped by
+    a row's place in its 16 bytes, so sums may differ by twice _lse_tol."""
+    T, V = 300, 5007
+    g = torch.Generator().manual_seed(i)
+    z = torch.randn(T, V, generator=g).to(DT[dtype]).cuda()
+    want = z.clone().requires_grad_()
+    lw = _three(want, i)
+    (gw,) = torch.autograd.grad(lw, want, torch.tensor(4.0, device="cuda"))
+
+    def held(pad, first):
+        wide = torch.full((T, V + pad), math.nan, device="cuda", dtype=DT[dtype])
+        wide[:, first:first + V] = z
+        return wide[:, first:first + V].requires_grad_()
+
+    flat = torch.full((T * V + 9,), math.nan, device="cuda", dtype=DT[dtype])
+    flat[3:3 + T * V] = z.reshape(-1)
+    for q in (held(49, 0), held(49, 5), held(3000, 7), flat[3:3 + T * V].view(T, V).requires_grad_()):
+        loss = _three(q, i)
+        assert abs(loss.item() - lw.item()) <= 0.1 * T * 2 * _lse_tol(V) + 2.0**-22 * abs(lw.item())
+        (gq,) = torch.autograd.grad(loss, q, torch.tensor(4.0, device="cuda"), retain_graph=True)
+        assert gq.shape == (T, V) and gq.isfinite().all()
+        assert (gq.float() - gw.float()).abs().max().item() <= 2.0**-7 * gw.abs().max().item()
+        (again,) = torch.autograd.grad(loss, q, torch.tensor(4.0, device="cuda"))
+        assert torch.equal(gq, again)
+    one = z[:1].expand(T, V).detach().requires_grad_()
+    loss = _three(one, i)
+    (gq,) = torch.autograd.grad(loss, one)
+    assert gq.shape == (T, V) and gq.isfinite().all()
