@@ -85,36 +85,25 @@ void set_upstream(sepx::VocabLossArgs& a, const c10::optional<at::Tensor>& up, c
   a.up = up->data_ptr<float>();
 }
 
-// num_valid >= 0: the rows in the loss, known on the host; negative: counted on the device.
-at::Tensor set_rows(sepx::VocabLossArgs& a, int op, int64_t num_valid, const at::Tensor& z) {
-  at::Tensor count;
-  if (num_valid >= 0) {
-    a.host_scale = 1.f / (float)std::max<int64_t>(num_valid, 1);
-  } else {
-    count = a.T > 0 ? at::empty({1}, z.options().dtype(at::kInt)) : at::zeros({1}, z.options().dtype(at::kInt));
-    a.count = count.data_ptr<int>();
-    sepx::vocab_count_rows(a, op, count.data_ptr<int>(), cs());
-  }
-  return count;
-}
-
 // Gradient of the logits, with rows at the same places in their 16 bytes as the logits' rows,
 // so that both move in whole vectors: the logits' row stride (where it costs little memory)
 // and the phase of their first row. Contiguous where the logits are.
 bool shares_stride(const at::Tensor& z) {
   return z.dim() == 2 && z.stride(0) >= z.size(1) && z.stride(0) <= z.size(1) + z.size(1) / 64 + 64;
 }
+int64_t phase_of(const at::Tensor& z) { return (int64_t)(reinterpret_cast<uintptr_t>(z.data_ptr()) % 16) / z.element_size(); }
 at::Tensor gradient_storage(const at::Tensor& z) {
   TORCH_CHECK(z.dim() == 2, "logits must be [T, V]");
+  if (z.is_contiguous() && phase_of(z) == 0) return at::empty(z.sizes(), z.options());
   return at::empty({z.size(0) * (shares_stride(z) ? z.stride(0) : z.size(1)) + 16 / z.element_size()}, z.options());
 }
 at::Tensor gradient_view(const at::Tensor& flat, const at::Tensor& z) {
-  const int64_t phase = (int64_t)(reinterpret_cast<uintptr_t>(z.data_ptr()) % 16) / z.element_size();
+  if (flat.dim() == 2) return flat;
   return flat.as_strided({z.size(0), z.size(1)}, {shares_stride(z) ? z.stride(0) : z.size(1), 1},
-                         flat.storage_offset() + phase);
+                         flat.storage_offset() + phase_of(z));
 }
 
-// Scratch of a call: records, partial sums and a ticket in one allocation.
+// Scratch of a call in one allocation: records, partial sums, a ticket and a count.
 at::Tensor set_scratch(sepx::VocabLossArgs& a, const at::Tensor& z, int64_t partial = 0) {
   const int64_t rec = (int64_t)a.T * sepx::kRowRecordBytes;
   const int64_t part = std::max<int64_t>(sepx::vocab_finish_blocks(a.T), partial) * 8;
@@ -124,6 +113,18 @@ at::Tensor set_scratch(sepx::VocabLossArgs& a, const at::Tensor& z, int64_t part
   a.partial = reinterpret_cast<double*>(p + rec);
   a.ticket = reinterpret_cast<unsigned int*>(p + rec + part);
   return s;
+}
+
+// num_valid >= 0: the rows in the loss, known on the host; negative: counted on the device,
+// into the scratch.
+void set_rows(sepx::VocabLossArgs& a, int op, int64_t num_valid) {
+  if (num_valid >= 0) {
+    a.host_scale = 1.f / (float)std::max<int64_t>(num_valid, 1);
+  } else {
+    int* count = reinterpret_cast<int*>(a.ticket + 1);
+    a.count = count;
+    sepx::vocab_count_rows(a, op, count, cs());
+  }
 }
 
 // Returns the loss; the gradient (of the loss times `up`) goes to `grad`, which may be the
@@ -148,7 +149,8 @@ at::Tensor distill_loss(const at::Tensor& z, const at::Tensor& ids, const at::Te
   set_upstream(a, up, z);
   const auto f32 = z.options().dtype(at::kFloat);
   at::Tensor loss = at::empty({}, f32);
-  const at::Tensor count = set_rows(a, sepx::kOpDistill, num_valid, z), scratch = set_scratch(a, z);
+  const at::Tensor scratch = set_scratch(a, z);
+  set_rows(a, sepx::kOpDistill, num_valid);
   a.loss = loss.data_ptr<float>();
   sepx::vocab_loss(a, sepx::kOpDistill, sms(), cs());
   return loss;
@@ -180,7 +182,8 @@ std::vector<at::Tensor> policy_loss(const at::Tensor& z, const at::Tensor& actio
   set_upstream(a, up, z);
   const auto f32 = z.options().dtype(at::kFloat);
   at::Tensor loss = at::empty({}, f32), logp = at::empty({a.T}, f32), kl = at::empty({a.T}, f32);
-  const at::Tensor count = set_rows(a, sepx::kOpPolicy, num_valid, z), scratch = set_scratch(a, z);
+  const at::Tensor scratch = set_scratch(a, z);
+  set_rows(a, sepx::kOpPolicy, num_valid);
   a.loss = loss.data_ptr<float>();
   a.logp = logp.data_ptr<float>();
   a.kl = kl.data_ptr<float>();
@@ -403,7 +406,8 @@ bool formed_in_forward(const at::Tensor& z) { return z.scalar_type() != at::kHal
 at::Tensor keep_gradient(AutogradContext* ctx, const at::Tensor& z) {
   const at::Tensor flat = gradient_storage(z), g = gradient_view(flat, z);
   ctx->saved_data["grad"] = flat;
-  ctx->saved_data["at"] = std::vector<int64_t>{g.size(0), g.size(1), g.stride(0), g.storage_offset()};
+  if (flat.dim() != 2)
+    ctx->saved_data["at"] = std::vector<int64_t>{g.size(0), g.size(1), g.stride(0), g.storage_offset()};
   return g;
 }
 at::Tensor take_formed(AutogradContext* ctx, const at::Tensor& up) {
@@ -412,6 +416,7 @@ at::Tensor take_formed(AutogradContext* ctx, const at::Tensor& up) {
   at::Tensor flat = kept.toTensor();
   kept = c10::IValue();
   scale_grad(flat, up);  // with what lies between the rows, which nothing reads
+  if (flat.dim() == 2) return flat;
   const auto at = ctx->saved_data["at"].toIntVector();
   return flat.as_strided({at[0], at[1]}, {at[2], 1}, at[3]);
 }
