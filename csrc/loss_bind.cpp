@@ -64,7 +64,8 @@ sepx::VocabLossArgs vocab_args(const at::Tensor& z, const c10::optional<at::Tens
   a.c2 = (float)c2;
   if ((double)a.c2 >= c2) a.c2 = std::nextafterf(a.c2, 0.f);
   a.c2_lo = (float)(c2 - (double)a.c2);
-  TORCH_CHECK(std::isfinite(c2) && a.c2 > 1e-30f && a.c2 < 1e30f, "temperature out of range");
+  // c2_lo is at least c2 2^-53: from 1e-20 on a normal number, which -inf times stays -inf.
+  TORCH_CHECK(std::isfinite(c2) && a.c2 > 1e-20f && a.c2 < 1e30f, "temperature out of range");
   a.tau = (float)tau;
   a.tau64 = tau;
   if (grad.has_value()) {

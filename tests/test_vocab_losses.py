@@ -526,7 +526,7 @@ def test_refusals():
     _refused(topk_distill_loss, z, k, t.expand(4, 2), match="shape of teacher_ids")
     _refused(topk_distill_loss, z, k.expand(4, 1025), t.expand(4, 1025), match="teacher entries")
     _refused(topk_distill_loss, z, k[:, :0], t[:, :0], match="teacher entries")
-    for tau in (0.0, -1.0, float("nan"), float("inf"), 1e-42):
+    for tau in (0.0, -1.0, float("nan"), float("inf"), 1e-42, 1e25):
         _refused(topk_distill_loss, z, k, t, temperature=tau, match="temperature")
     _refused(topk_distill_loss, z, k, t, num_valid=-2, match="num_valid")
     _refused(clipped_policy_loss, z, i, f, f, match="CUDA")
