@@ -398,7 +398,11 @@ __global__ void __launch_bounds__(kWarps * 32) router_balance_bwd_kernel(const R
     pe = lane < a.k && a.dw ? fast_exp(pe - mx) * inv : 0.f;
     float dot = 0.f;  // sum p g: zero over the chosen experts where their weights sum to 1
     if (a.dw) {
-      if (a.renorm) {  // w = p / S: d / dp_i = (g_i - sum_j g_j w_j) / S
+      if (a.renorm) {
+        // w = p / S: d / dp_i = (g_i - sum_j g_j w_j) / S. The weights sum to 1, so the g may be
+        // counted from the first choice's: where it has nearly all the weight (all of it at
+        // k = 1, where the result is 0) nothing large is left to cancel.
+        ge -= __shfl_sync(0xffffffffu, ge, 0);
         float S = pe, gw = ge * pe;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {

@@ -231,3 +231,41 @@ def test_router_refusals():
     refused(x, 2, valid=torch.ones(4), match="valid")
     refused(x, 2, bias=torch.zeros(7), match="bias")
     refused(x, 2, bias=torch.zeros(8).double(), match="bias")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("T,E", [(1, 1), (40, 13), (600, 128), (90, 512)])
+def test_one_choice_with_weight_one_gets_no_gradient_through_it(T, E, dtype):
+    """k = 1, renormalised: the weight is 1 whatever the logits are, so the gradient is that
+    of the balance loss alone, to the bit, however small it is beside the weights'."""
+    from spec_ep.ops.router import router_topk_balanced
+
+    x, g = _inputs(T, E, dtype, T + E)
+    dw, up = 100.0 * torch.randn(T, 1, generator=g).cuda(), torch.tensor(0.01, device="cuda")
+    w, _, loss, _ = router_topk_balanced(x, 1)
+    assert (w == 1.0).all()
+    (both,) = torch.autograd.grad([w, loss], x, [dw, up], retain_graph=True)
+    (alone,) = torch.autograd.grad(loss, x, up)
+    assert torch.equal(both, alone)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [4.0, 12.0])
+def test_gradient_of_nearly_certain_choices(d):
+    """Two choices whose logits lie d apart: dx_0 = w_0 w_1 (dw_0 - dw_1) = -dx_1, small
+    beside dw. Relative errors: d 2^-23 of the exponential's argument (the product's rounding
+    and the constant's, each d 2^-24), 2 * 2^-23 of the exponential, and below 20 roundings
+    of 2^-24 or divisions of 2^-23 from the sums, weights and products."""
+    from spec_ep.ops.router import router_topk_balanced
+
+    T = 256
+    g = torch.Generator().manual_seed(int(d))
+    x = torch.tensor([0.0, -d]).repeat(T, 1).cuda().requires_grad_()
+    dw = torch.randn(T, 2, generator=g).cuda()
+    w, _, _, _ = router_topk_balanced(x, 2)
+    (gx,) = torch.autograd.grad(w, x, dw)
+    w1 = 1.0 / (1.0 + math.exp(d))
+    want = w1 * (1.0 - w1) * (dw[:, 0] - dw[:, 1]).double()
+    for got, sign in ((gx[:, 0], 1.0), (gx[:, 1], -1.0)):
+        assert ((got.double() - sign * want).abs() <= want.abs() * (d + 22) * 2.0**-23).all()
