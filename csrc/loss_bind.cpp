@@ -62,8 +62,10 @@ sepx::VocabLossArgs vocab_args(const at::Tensor& z, const c10::optional<at::Tens
   // in two parts, the second above 0: a logit of -infinity has to stay one in both products
   const double c2 = 1.4426950408889634 / tau;
   a.c2 = (float)c2;
-  if ((double)a.c2 >= c2) a.c2 = std::nextafterf(a.c2, 0.f);
-  a.c2_lo = (float)(c2 - (double)a.c2);
+  int exponent = 0;
+  const double bits = std::frexp(c2, &exponent) * 4096;  // 2048 <= bits < 4096
+  a.c2_hi = (float)std::ldexp(std::ceil(bits) - 1, exponent - 12);
+  a.c2_lo = (float)(c2 - (double)a.c2_hi);
   // c2_lo is at least c2 2^-53: from 1e-20 on a normal number, which -inf times stays -inf.
   TORCH_CHECK(std::isfinite(c2) && a.c2 > 1e-20f && a.c2 < 1e30f, "temperature out of range");
   a.tau = (float)tau;

@@ -217,15 +217,17 @@ __device__ __forceinline__ int64_t load_id(const void* p, int64_t i, bool is64) 
 
 // ------------------------------------------------------------------------------------
 // Exponentials of a row: 2^(z c2 - M2), c2 = log2(e) / tau in two parts (the rounding of one
-// fp32 would show in log-probabilities: 1.3e-8 of a token's distance from the mean logit),
-// M2 = m c2 of a reference m (the row's maximum, or near it), rounded to a whole number: sums
+// fp32 would show in log-probabilities: 1.3e-8 of a token's distance from the mean logit). The
+// first part has 12 bits: its product with a 16-bit logit is exact, and the second part's
+// product is not so small beside the first result that rounding always drops it, which left a
+// mean error of 4e-8 per token. M2 = m c2 of a reference m (the row's maximum, or near it), rounded to a whole number: sums
 // against different references are joined by powers of two, exactly. Where m c2 leaves fp32
 // (rows whose largest value is the type's lowest or highest), the difference z - m comes
 // first.
 // ------------------------------------------------------------------------------------
 constexpr float kFarM2 = 1e37f;
 struct C2 {
-  float hi, lo;
+  float all, hi, lo;  // all: one fp32, for references and gradients
 };
 struct Expo {
   C2 c2;
@@ -234,17 +236,17 @@ struct Expo {
   __device__ __forceinline__ Expo(C2 c2_, float m_) {
     c2 = c2_;
     m = m_;
-    M2 = rintf(m_ * c2.hi);
+    M2 = rintf(m_ * c2.all);
     far = !(fabsf(M2) <= kFarM2);
   }
   __device__ __forceinline__ float arg(float z) const {
-    return far ? (z - m) * c2.hi : fmaf(z, c2.lo, fmaf(z, c2.hi, -M2));
+    return far ? (z - m) * c2.all : fmaf(z, c2.lo, fmaf(z, c2.hi, -M2));
   }
   __device__ __forceinline__ float operator()(float z) const { return ex2(arg(z)); }
   // a sum against reference r, against this reference instead
   __device__ __forceinline__ float join(float r, float s) const {
     if (r == -INFINITY) return s;  // nothing yet: 0 (or NaN, which stays)
-    return s * ex2(far ? (r - m) * c2.hi : rintf(r * c2.hi) - M2);
+    return s * ex2(far ? (r - m) * c2.all : rintf(r * c2.all) - M2);
   }
 };
 
@@ -257,11 +259,18 @@ __device__ __forceinline__ float max_of(const uint4& raw, float ref) {
   for (int i = 0; i < Elem<T>::N; ++i) ref = fmaxf(ref, o[i]);
   return ref;
 }
+// The fast sum's terms are 2^kShift smaller, so that their arguments stay below 0 for values
+// up to 5.5 tau above a thread's reference: there the hardware exponential's mean error is one
+// number (measured: -5.0e-8 relative over [-9, 0), -5.1e-8 down to -25; +3.3e-8 above 0), which
+// the 64-bit logarithm of a row's sum takes out. Left in, it adds up over a sequence's tokens
+// while the other errors average out.
+constexpr float kShift = 8.f, kShiftUp = 256.f, kShiftDown = 1.f / 256.f;
+constexpr double kExpMeanError = -5.05e-8;
 // What the fast form z c2 + R adds for reference m: NaN (or infinity) where the sum has to
-// take the careful form.
+// take the careful form, also where M2 + kShift might not be exact.
 __device__ __forceinline__ float reference(float m, C2 c2) {
   const Expo w(c2, m);
-  return m == -INFINITY ? INFINITY : w.far ? __int_as_float(0x7fffffff) : -w.M2;
+  return m == -INFINITY ? INFINITY : !(fabsf(w.M2) <= 8388608.f) ? __int_as_float(0x7fffffff) : -w.M2 - kShift;
 }
 
 // The careful forms of the two passes over n vectors `step` apart in shared memory: a sum
@@ -534,7 +543,7 @@ __global__ void __launch_bounds__(512) vocab_row_kernel(const VocabLossArgs a) {
 #pragma unroll
     for (int i = 0; i < N; ++i) mx = fmaxf(mx, o[i]);
   }
-  const Expo x(C2{a.c2, a.c2_lo}, block_max(mx, red));
+  const Expo x(C2{a.c2, a.c2_hi, a.c2_lo}, block_max(mx, red));
   for (int j = threadIdx.x; j < z.nv; j += blockDim.x) {
     float o[N];
     Elem<T>::unpack(z.load(j), o);
@@ -802,9 +811,9 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
         __syncwarp();
         if (!wait_exchange(&sh.pairs_full[x & 1], x >> 1)) break;
         float sum;
-        join_pairs(sh.pairs[x & 1], C * CW, C2{a.c2, a.c2_lo}, lane, &m, &sum);
+        join_pairs(sh.pairs[x & 1], C * CW, C2{a.c2, a.c2_hi, a.c2_lo}, lane, &m, &sum);
         if (a.grad) {
-          A = row_factor<OP>(a, token, Expo(C2{a.c2, a.c2_lo}, m), sum, factor);
+          A = row_factor<OP>(a, token, Expo(C2{a.c2, a.c2_hi, a.c2_lo}, m), sum, factor);
           As = A / sum;
         }
         if (lane == 0) {
@@ -823,7 +832,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
       if constexpr (OP == kOpDistill) {
         if (!wait(&sh.dense_done[e], lap)) break;
         if (a.grad && token.state != kRowOff) {  // the entries' values replace the dense ones
-          const Expo w(C2{a.c2, a.c2_lo}, m);
+          const Expo w(C2{a.c2, a.c2_hi, a.c2_lo}, m);
           const Entries s = entries(e);
           const RowVec<T> z = row_z(t);
           int j0, j1;
@@ -854,8 +863,8 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
       for (int i = 0; i < N; ++i) o[i] = -INFINITY;
       none = Elem<T>::pack(o);
     }
-    const C2 c2 = {a.c2, a.c2_lo};
-    const F2 cc = f2(a.c2, a.c2), cl = f2(a.c2_lo, a.c2_lo);
+    const C2 c2 = {a.c2, a.c2_hi, a.c2_lo};
+    const F2 cc = f2(a.c2, a.c2), ch = f2(a.c2_hi, a.c2_hi), cl = f2(a.c2_lo, a.c2_lo);
     auto piece_at = [&](int sl) { return reinterpret_cast<const uint4*>(ring + (size_t)sl * kPieceBytes) + tid; };
     int slot = 0, turn = 0, grad_slot = 0, e = 0, lap = 0, x = 0;
     // the row that is summed: done of np pieces
@@ -909,7 +918,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
 #pragma unroll
           for (int i = 0; i < N; i += 2) {
             const F2 z2 = f2(o[i], o[i + 1]);
-            acc[(i >> 1) & 1] = add2(acc[(i >> 1) & 1], ex2_2(fma2(z2, cl, fma2(z2, cc, nR2))));
+            acc[(i >> 1) & 1] = add2(acc[(i >> 1) & 1], ex2_2(fma2(z2, cl, fma2(z2, ch, nR2))));
           }
         };
         auto total = [&](F2 (&acc)[2]) {
@@ -918,9 +927,9 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
           return sum + (ax + ay);
         };
         auto add_carefully = [&](const uint4* piece, int n, bool first) {
-          const float2 r = careful_sum<T>(piece, n, Cfg::Lanes, c2, first ? -INFINITY : ref, sum);
+          const float2 r = careful_sum<T>(piece, n, Cfg::Lanes, c2, first ? -INFINITY : ref, sum * kShiftUp);
           ref = r.x;
-          sum = r.y;
+          sum = r.y * kShiftDown;
           const float R = reference(ref, c2);
           nR2 = f2(R, R);
         };
@@ -1084,7 +1093,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
       // may only leave once this block has joined row x - 1.
       if (!a.grad && x > 0 && !wait(&sh.factor_full[(x - 1) & 1], (x - 1) >> 1)) goto out;
       const float mw = warp_max(ref);
-      sum = warp_sum(Expo(c2, mw).join(ref, sum));
+      sum = warp_sum(Expo(c2, mw).join(ref, sum * kShiftUp));
       if (C == 1) {
         if (lane == 0) {
           sh.pairs[x & 1][warp] = make_float2(mw, sum);
@@ -1137,11 +1146,11 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Voca
   float loss = 0.f;
   if (t < a.T) {
     const RowRecord r = reinterpret_cast<const RowRecord*>(a.records)[t];
-    const Expo x(C2{a.c2, a.c2_lo}, r.m);
+    const Expo x(C2{a.c2, a.c2_hi, a.c2_lo}, r.m);
     double lp = 0.0;  // ln q of the token (of the entry that zref is from)
     if (r.state == kRowOn)
       lp = (x.far ? ((double)r.z - (double)r.m) / a.tau64 : (double)r.z / a.tau64 - (double)x.M2 * ln2) -
-           log((double)r.sum);
+           log((double)r.sum) + kExpMeanError;
     if constexpr (OP == kOpDistill) {
       if (r.state == kRowOn) loss = (float)((double)a.tau * a.tau * (r.base - (double)r.weight * lp));
       else if (r.state == kRowBad) loss = nan;
@@ -1320,7 +1329,7 @@ __global__ void __launch_bounds__(kGradThreads) preference_grad_kernel(const Voc
     return;
   }
   const float A = -coef * *a.up, As = A / l.y;
-  const C2 c2 = {a.c2, a.c2_lo};
+  const C2 c2 = {a.c2, a.c2_hi, a.c2_lo};
   const Expo x(c2, l.x);
   const bool plain = same && !x.far;
   const F2 cc = f2(a.c2, a.c2), nM2 = f2(-x.M2, -x.M2), As2 = f2(As, As);

@@ -22,7 +22,7 @@ struct VocabLossArgs {
   int64_t grad_stride = 0;
   int dtype = kVocabBf16;
   int T = 0, V = 0;
-  float c2 = 0.f, c2_lo = 0.f;  // log2(e) / temperature, and what its rounding left
+  float c2 = 0.f, c2_hi = 0.f, c2_lo = 0.f;  // log2(e) / temperature; its first 12 bits and the rest
   float tau = 1.f;           // temperature, and unrounded
   double tau64 = 1.0;
   float host_scale = 1.f;    // 1 / rows in the loss, when the host knows it ...

@@ -505,6 +505,24 @@ def test_row_offsets_pass_32_bits():
     assert not g[:-1].any() and g[-1, 77].item() > 0
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("tau", [1.0, 2.0])
+def test_log_probabilities_have_no_mean_error(tau):
+    """What all tokens of a sequence are off by alike adds up in its log-ratio. Single errors
+    here: the output's rounding (|logp| < 16: at most 2^-21, 2^-21 / sqrt 3 = 2.8e-7 rms) and
+    that of the row's sum (below 2e-7 rms), together 3.4e-7; over 8192 rows their mean stays
+    below 4 * 3.4e-7 / sqrt(8192) = 1.5e-8, and the exponential's mean error is known to 1e-9."""
+    from spec_ep.ops.loss import token_logp
+
+    T, V = 8192, 4096
+    g = torch.Generator("cuda").manual_seed(5)
+    z = 2.0 * torch.randn(T, V, generator=g, device="cuda")
+    y = torch.randint(0, V, (T,), generator=g, device="cuda")
+    want = torch.log_softmax(z.double() / tau, 1).gather(1, y[:, None])[:, 0]
+    off = token_logp(z, y.int(), tau).double() - want
+    assert abs(off.mean().item()) < 2e-8
+
+
 # -------------------------------------------------------------------------- refusals, CPU
 def _refused(f, *a, match, **kw):
     with pytest.raises((RuntimeError, ValueError), match=match):
