@@ -220,10 +220,10 @@ __device__ __forceinline__ int64_t load_id(const void* p, int64_t i, bool is64) 
 // fp32 would show in log-probabilities: 1.3e-8 of a token's distance from the mean logit). The
 // first part has 12 bits: its product with a 16-bit logit is exact, and the second part's
 // product is not so small beside the first result that rounding always drops it, which left a
-// mean error of 4e-8 per token. M2 = m c2 of a reference m (the row's maximum, or near it), rounded to a whole number: sums
-// against different references are joined by powers of two, exactly. Where m c2 leaves fp32
-// (rows whose largest value is the type's lowest or highest), the difference z - m comes
-// first.
+// mean error of 4e-8 per token. M2 = m c2 of a reference m (the row's maximum, or near it),
+// rounded to a whole number: sums against different references are joined by powers of two,
+// exactly. Where m c2 leaves fp32 (rows whose largest value is the type's lowest or highest),
+// the difference z - m comes first.
 // ------------------------------------------------------------------------------------
 constexpr float kFarM2 = 1e37f;
 struct C2 {
@@ -592,7 +592,7 @@ __global__ void __launch_bounds__(512) vocab_row_kernel(const VocabLossArgs a) {
 // Every wait is bounded; one that runs out turns the call's outputs into NaN.
 //
 // What bounds it: memory would take 380 us for 4096 x 151936 bf16 with gradients (2.5 GB at
-// 6.55 TB/s); measured 487-495 us, 5.1 TB/s, with every byte moved once (a capture of 1024
+// 6.55 TB/s); measured 484-502 us, 5.1 TB/s, with every byte moved once (a capture of 1024
 // rows reads 313 MB and writes 311 MB, the last 55 MB of it still in L2). The two
 // exponentials per logit keep the special-function unit 57% busy and the schedulers 48%: the
 // consumers' own latencies (a wait costs ~120 cycles, a row's exchange of sums ~2500, hidden
