@@ -222,10 +222,11 @@ __device__ __forceinline__ int64_t load_id(const void* p, int64_t i, bool is64) 
 // product is not so small beside the first result that rounding always drops it, which left a
 // mean error of 4e-8 per token. M2 = m c2 of a reference m (the row's maximum, or near it),
 // rounded to a whole number: sums against different references are joined by powers of two,
-// exactly. Where m c2 leaves fp32 (rows whose largest value is the type's lowest or highest),
-// the difference z - m comes first.
+// exactly. The fused products form z c2 - M2 to 2^-36 of |M2| (the second part's own rounding),
+// which is 2^-19 where |M2| is 2^17; beyond that (rows of mask values such as -1e9 or the
+// type's lowest, logits far from 0) the difference z - m comes first, and M2 is not used.
 // ------------------------------------------------------------------------------------
-constexpr float kFarM2 = 1e37f;
+constexpr float kFarM2 = 131072.f;
 struct C2 {
   float all, hi, lo;  // all: one fp32, for references and gradients
 };
@@ -240,13 +241,20 @@ struct Expo {
     far = !(fabsf(M2) <= kFarM2);
   }
   __device__ __forceinline__ float arg(float z) const {
-    return far ? (z - m) * c2.all : fmaf(z, c2.lo, fmaf(z, c2.hi, -M2));
+    if (far) {
+      const float d = z - m;
+      return fmaf(d, c2.lo, d * c2.hi);
+    }
+    return fmaf(z, c2.lo, fmaf(z, c2.hi, -M2));
   }
   __device__ __forceinline__ float operator()(float z) const { return ex2(arg(z)); }
   // a sum against reference r, against this reference instead
   __device__ __forceinline__ float join(float r, float s) const {
     if (r == -INFINITY) return s;  // nothing yet: 0 (or NaN, which stays)
-    return s * ex2(far ? (r - m) * c2.all : rintf(r * c2.all) - M2);
+    const Expo w(c2, r);
+    // how much of a power of two r lies above m; against a far reference no whole number
+    const float up = w.far ? arg(r) : far ? -w.arg(m) : w.M2 - M2;
+    return s * ex2(up);
   }
 };
 
@@ -267,10 +275,10 @@ __device__ __forceinline__ float max_of(const uint4& raw, float ref) {
 constexpr float kShift = 8.f, kShiftUp = 256.f, kShiftDown = 1.f / 256.f;
 constexpr double kExpMeanError = -5.05e-8;
 // What the fast form z c2 + R adds for reference m: NaN (or infinity) where the sum has to
-// take the careful form, also where M2 + kShift might not be exact.
+// take the careful form.
 __device__ __forceinline__ float reference(float m, C2 c2) {
   const Expo w(c2, m);
-  return m == -INFINITY ? INFINITY : !(fabsf(w.M2) <= 8388608.f) ? __int_as_float(0x7fffffff) : -w.M2 - kShift;
+  return m == -INFINITY ? INFINITY : w.far ? __int_as_float(0x7fffffff) : -w.M2 - kShift;
 }
 
 // The careful forms of the two passes over n vectors `step` apart in shared memory: a sum
