@@ -228,8 +228,11 @@ __device__ __forceinline__ int64_t load_id(const void* p, int64_t i, bool is64) 
 // ------------------------------------------------------------------------------------
 constexpr float kFarM2 = 131072.f;
 struct C2 {
-  float all, hi, lo;  // all: one fp32, for references and gradients
+  float all, hi, lo;  // all: one fp32, for references
 };
+// z c2 + R for two z, in sums and gradients alike: a gradient with the constant in one fp32
+// would be off by 1.3e-8 of z against its row's sum.
+__device__ __forceinline__ F2 arg2(F2 z, F2 hi, F2 lo, F2 R) { return fma2(z, lo, fma2(z, hi, R)); }
 struct Expo {
   C2 c2;
   float m, M2;
@@ -872,7 +875,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
       none = Elem<T>::pack(o);
     }
     const C2 c2 = {a.c2, a.c2_hi, a.c2_lo};
-    const F2 cc = f2(a.c2, a.c2), ch = f2(a.c2_hi, a.c2_hi), cl = f2(a.c2_lo, a.c2_lo);
+    const F2 ch = f2(a.c2_hi, a.c2_hi), cl = f2(a.c2_lo, a.c2_lo);
     auto piece_at = [&](int sl) { return reinterpret_cast<const uint4*>(ring + (size_t)sl * kPieceBytes) + tid; };
     int slot = 0, turn = 0, grad_slot = 0, e = 0, lap = 0, x = 0;
     // the row that is summed: done of np pieces
@@ -926,7 +929,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
 #pragma unroll
           for (int i = 0; i < N; i += 2) {
             const F2 z2 = f2(o[i], o[i + 1]);
-            acc[(i >> 1) & 1] = add2(acc[(i >> 1) & 1], ex2_2(fma2(z2, cl, fma2(z2, ch, nR2))));
+            acc[(i >> 1) & 1] = add2(acc[(i >> 1) & 1], ex2_2(arg2(z2, ch, cl, nR2)));
           }
         };
         auto total = [&](F2 (&acc)[2]) {
@@ -1038,7 +1041,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
           Elem<T>::unpack(raw, o);
 #pragma unroll
           for (int i = 0; i < N; i += 2)
-            split(mul2(As2, ex2_2(fma2(f2(o[i], o[i + 1]), cc, nM2))), o[i], o[i + 1]);
+            split(mul2(As2, ex2_2(arg2(f2(o[i], o[i + 1]), ch, cl, nM2))), o[i], o[i + 1]);
           *reinterpret_cast<uint4*>(to) = Elem<T>::pack(o);
         };
         auto free_slot = [&] {
@@ -1340,7 +1343,7 @@ __global__ void __launch_bounds__(kGradThreads) preference_grad_kernel(const Voc
   const C2 c2 = {a.c2, a.c2_hi, a.c2_lo};
   const Expo x(c2, l.x);
   const bool plain = same && !x.far;
-  const F2 cc = f2(a.c2, a.c2), nM2 = f2(-x.M2, -x.M2), As2 = f2(As, As);
+  const F2 ch = f2(a.c2_hi, a.c2_hi), cl = f2(a.c2_lo, a.c2_lo), nM2 = f2(-x.M2, -x.M2), As2 = f2(As, As);
   for (int base = j0; base < j1; base += kGradThreads * kGradVecs) {
     uint4 raw[kGradVecs];
 #pragma unroll
@@ -1357,7 +1360,7 @@ __global__ void __launch_bounds__(kGradThreads) preference_grad_kernel(const Voc
         Elem<T>::unpack(raw[v], o);
 #pragma unroll
         for (int i = 0; i < N; i += 2)
-          split(mul2(As2, ex2_2(fma2(f2(o[i], o[i + 1]), cc, nM2))), o[i], o[i + 1]);
+          split(mul2(As2, ex2_2(arg2(f2(o[i], o[i + 1]), ch, cl, nM2))), o[i], o[i + 1]);
         __stcs(reinterpret_cast<uint4*>(g.p + z.first(j)), Elem<T>::pack(o));
       } else {
         const uint4 r = z.load(j);
