@@ -217,8 +217,8 @@ void set_offsets(sepx::VocabLossArgs& a, const at::Tensor& offsets, const at::Te
   a.num_seq = (int)offsets.size(0) - 1;
 }
 
-// Returns (loss, rewards [2 * pairs], logp [T], rows [4, T]: the rows' lse as T pairs, then
-// d loss / d logp, then scratch). With `grad` (may be the logits), d logp / d logits of each
+// Returns (loss, rewards [2 * pairs], logp [T], rows [5, T]: the rows' lse as T pairs, then
+// d loss / d logp, then scratch, then the sums without the labels' terms). With `grad` (may be the logits), d logp / d logits of each
 // row is written there.
 std::vector<at::Tensor> preference_fwd(const at::Tensor& z, const at::Tensor& labels, const at::Tensor& offsets,
                                        const at::Tensor& ref_logp, double beta, double eps,
@@ -237,12 +237,13 @@ std::vector<at::Tensor> preference_fwd(const at::Tensor& z, const at::Tensor& la
   q.pairs = a.num_seq / 2;
   const auto f32 = z.options().dtype(at::kFloat);
   at::Tensor loss = at::empty({}, f32), rewards = at::empty({2 * (int64_t)q.pairs}, f32);
-  at::Tensor logp = at::empty({a.T}, f32), rows = at::empty({4, a.T}, f32);
+  at::Tensor logp = at::empty({a.T}, f32), rows = at::empty({5, a.T}, f32);
   const at::Tensor scratch = set_scratch(a, z, q.pairs);
   a.logp = logp.data_ptr<float>();
   a.lse = rows.data_ptr<float>();
   a.row_coef = a.lse + 2 * (int64_t)a.T;
   a.ratio = a.lse + 3 * (int64_t)a.T;
+  a.rest = a.lse + 4 * (int64_t)a.T;
   a.ref_logp = ref_logp.data_ptr<float>();
   if (a.T > 0) sepx::vocab_loss(a, sepx::kOpLogp, sms(), cs());
   else if (q.pairs > 0) C10_CUDA_CHECK(cudaMemsetAsync(a.ticket, 0, sizeof(int), cs()));
@@ -269,7 +270,7 @@ at::Tensor preference_grad(const at::Tensor& z, const at::Tensor& labels, const 
   auto a = vocab_args(z, grad, 1.0);
   req_rows(labels, z, "labels");
   TORCH_CHECK(rows.device() == z.device() && rows.scalar_type() == at::kFloat && rows.is_contiguous() &&
-                  rows.numel() == 4 * z.size(0),
+                  rows.numel() == 5 * z.size(0),
               "rows must be the forward's");
   set_offsets(a, offsets, z);
   a.ids64 = ids_are_64(labels, "labels");
@@ -277,6 +278,7 @@ at::Tensor preference_grad(const at::Tensor& z, const at::Tensor& labels, const 
   const c10::cuda::CUDAGuard guard(z.device());
   a.labels = labels.data_ptr();
   a.lse = rows.data_ptr<float>();
+  a.rest = a.lse + 4 * (int64_t)a.T;
   set_upstream(a, up, z);
   sepx::preference_grad(a, a.lse + 2 * (int64_t)a.T, cs());
   return grad;

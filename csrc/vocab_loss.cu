@@ -18,6 +18,7 @@
 #include <mutex>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "kernels.h"
 #include "sm100.cuh"
@@ -270,12 +271,22 @@ __device__ __forceinline__ float max_of(const uint4& raw, float ref) {
   for (int i = 0; i < Elem<T>::N; ++i) ref = fmaxf(ref, o[i]);
   return ref;
 }
-// The fast sum's terms are 2^kShift smaller, so that their arguments stay below 0 for values
-// up to 5.5 tau above a thread's reference: there the hardware exponential's mean error is one
-// number (measured: -5.0e-8 relative over [-9, 0), -5.1e-8 down to -25; +3.3e-8 above 0), which
-// the 64-bit logarithm of a row's sum takes out. Left in, it adds up over a sequence's tokens
-// while the other errors average out.
-constexpr float kShift = 8.f, kShiftUp = 256.f, kShiftDown = 1.f / 256.f;
+// A row's sum leaves out the token that the outputs are about (the chosen token, the teacher's
+// entry of largest logit): its own term joins in 64 bits, so that ln q = -log(1 + rest / own)
+// and 1 - q = rest / (own + rest) keep their digits where q is near 1, and ln q is never above 0.
+//
+// The other terms are formed 2^kShift smaller, so that their arguments stay below 0 for values
+// up to 6.9 tau above the reference (beyond, the reference moves): there the hardware
+// exponential's mean error is one number (measured: -5.0e-8 relative over [-9, 0), -5.1e-8 down
+// to -25; +3.3e-8 above 0), which is taken out of each row's sum in 64 bits. Left in, it adds up
+// over a sequence's tokens while the other errors average out. It is a mean over arguments with
+// spread fractions: in a row of equal logits (or at a temperature that makes them equal) it may
+// itself be the error, below half a rounding of the row's log-probability.
+constexpr float kShift = 10.f, kShiftUp = 1024.f;
+// What a thread's sum of shifted terms may grow to before its reference moves. A thread has at
+// most kMaxSlots * 16 terms of a row, in the present shapes 208, so terms near the reference
+// stay below 208 * 2^(0.5 - kShift) = 0.29; one with an argument above 0 does not.
+constexpr float kMostSum = 1.f;
 constexpr double kExpMeanError = -5.05e-8;
 // What the fast form z c2 + R adds for reference m: NaN (or infinity) where the sum has to
 // take the careful form.
@@ -297,9 +308,23 @@ __device__ __noinline__ float2 careful_sum(const uint4* v, int n, int step, C2 c
     float o[Elem<T>::N];
     Elem<T>::unpack(v[k * step], o);
 #pragma unroll
-    for (int i = 0; i < Elem<T>::N; ++i) sum += w(o[i]);
+    for (int i = 0; i < Elem<T>::N; ++i) sum += ex2(w.arg(o[i]) - kShift);
   }
   return make_float2(m, sum);
+}
+// Sets an element of a vector to -infinity: it adds nothing to the sum.
+template <typename T>
+__device__ __noinline__ void blank(uint4* v, int element) {
+  const uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;
+  const int at = element * (int)sizeof(T), shift = (at % 4) * 8;
+  const uint32_t mask = sizeof(T) == 4 ? 0xffffffffu : 0xffffu << shift;
+  uint4 o = *v;
+  auto put = [&](uint32_t& w, int i) { w = at / 4 == i ? (w & ~mask) | (none << shift) : w; };
+  put(o.x, 0);
+  put(o.y, 1);
+  put(o.z, 2);
+  put(o.w, 3);
+  *v = o;
 }
 template <typename T>
 __device__ __noinline__ void careful_store(const uint4* v, T* row, int V, int64_t e0, C2 c2, float m, float As) {
@@ -349,11 +374,12 @@ enum RowState : int { kRowOff = 0, kRowOn = 1, kRowBad = 2 };
 
 struct RowRecord {
   double base;    // distillation: sum P (ln P - (z - zref) / tau)
-  float m, sum;   // the row's reference and sum of exponentials
+  float m, rest;  // the row's reference, and its sum of exponentials without the token's
   float z;        // the token's logit; distillation: zref
   float weight;   // distillation: sum P
   int state;
-  int pad;
+  int id;         // the token; distillation: the first id with zref, -1 where no entry has a
+                  // logit above -infinity (zref is 0 then, and the sum complete)
 };
 static_assert(sizeof(RowRecord) == kRowRecordBytes, "scratch size");
 
@@ -385,7 +411,8 @@ __device__ __forceinline__ float weight_of(const Entries& s, int id) {
   return P;
 }
 
-// What the gradient takes from one token (policy, log-probability).
+// What the sum and the gradient take from one token (distillation: the id and zref of the
+// record).
 struct Token {
   int state, id;
   float z, adv, old_logp, ref_logp;  // z: its logit
@@ -446,7 +473,14 @@ __device__ __forceinline__ int load_entries(const VocabLossArgs& a, int t, const
   }
   const float lsum = logf(warp_sum(sum));
   zref = warp_max(zref);
-  if (zref == -INFINITY) zref = 0.f;
+  int first = 0x7fffffff;  // the lowest id with zref
+  for (int k = lane; k < K; k += 32)
+    if (s.id[k] >= 0 && s.z[k] == zref) first = min(first, s.id[k]);
+  first = __reduce_min_sync(0xffffffffu, first);
+  if (zref == -INFINITY) {
+    zref = 0.f;
+    first = -1;
+  }
   double base = 0.0;
   float weight = 0.f;
   for (int k = lane; k < K; k += 32) {
@@ -464,6 +498,7 @@ __device__ __forceinline__ int load_entries(const VocabLossArgs& a, int t, const
   rec->base = base;
   rec->weight = warp_sum(weight);
   rec->z = zref;
+  rec->id = first;
   rec->state = bad ? kRowBad : kRowOn;
   __syncwarp();
   return rec->state;
@@ -498,15 +533,41 @@ __device__ __forceinline__ float loss_factor(const VocabLossArgs& a) {
   return (a.count ? 1.f / (float)max(*a.count, 1) : a.host_scale) * (a.up ? *a.up : 1.f);
 }
 
-// The factor A of the gradient A (q - P) of a row in the loss. x: the row's exponentials,
-// sum: theirs; g: loss_factor.
+// ln q of a token with logit z from the row's reference and the sum of the other terms (apart
+// false: of all terms). Formed in 64 bits: in fp32 the rounding of ln(sum) near 12 alone is
+// 5e-7, and a sequence's log-ratio sums hundreds.
+__device__ __noinline__ double row_logp(C2 c2, float z, float m, float rest, bool apart) {
+  const Expo x(c2, m);
+  const double c = (double)c2.hi + (double)c2.lo;
+  const double arg = x.far ? ((double)z - (double)m) * c : (double)z * c - (double)x.M2;  // the token's own term is 2^arg
+  const double r = (double)rest * (1.0 - kExpMeanError), own = apart ? exp2(arg) : 0.0;
+  return r < own ? -log1p(r / own) : arg * 0.69314718055994530942 - log(r + own);
+}
+
+// The same to fp32's accuracy (a 64-bit logarithm here would delay every row by 1000 cycles:
+// 427 us instead of 397 us for 4096 x 151936). The policy loss and its gradient both take the
+// ratio, and so their side of the clip, from these bits.
+__device__ __forceinline__ double quick_logp(C2 c2, float z, float m, float rest) {
+  const Expo x(c2, m);
+  const float own = x(z);
+  if (rest < own) return -log1pf(rest / own);
+  const double c = (double)c2.hi + (double)c2.lo;
+  const double arg = x.far ? ((double)z - (double)m) * c : (double)z * c - (double)x.M2;
+  int e;
+  const float f = frexpf(rest + own, &e);  // what is left is the logarithm of a number in [1/2, 1)
+  return (arg - e) * 0.69314718055994530942 - logf(f);
+}
+
+// The factor A of the gradient A (q - P) of a row in the loss, from the row's reference and the
+// sum of the other tokens' terms; g: loss_factor.
 template <int OP>
-__device__ __forceinline__ float row_factor(const VocabLossArgs& a, const Token& k, const Expo& x, float sum, float g) {
+__device__ __forceinline__ float row_factor(const VocabLossArgs& a, const Token& k, float m, float rest, float g) {
   if (k.state == kRowBad) return __int_as_float(0x7fffffff);
   if constexpr (OP == kOpLogp) return -1.f;
   if constexpr (OP == kOpDistill) return a.tau * g;
-  const float lp = x.arg(k.z) * 0.69314718055994531f - logf(sum);
-  return -policy_term(a, k.adv, expf(lp - k.old_logp), k.ref_logp - lp, a.ref_logp != nullptr).dl / a.tau * g;
+  const double lp = quick_logp(C2{a.c2, a.c2_hi, a.c2_lo}, k.z, m, rest);
+  return -policy_term(a, k.adv, expf((float)(lp - (double)k.old_logp)), (float)((double)k.ref_logp - lp),
+                      a.ref_logp != nullptr).dl / a.tau * g;
 }
 
 // Rows longer than a cluster's shared memory: one block per row, which reads the row for its
@@ -527,10 +588,13 @@ __global__ void __launch_bounds__(512) vocab_row_kernel(const VocabLossArgs a) {
     Token k = {};
     if constexpr (OP == kOpDistill) {
       k.state = load_entries(a, t, z.p, s, lane, &r);
+      k.id = r.id;
+      k.z = r.z;
     } else {
       k = load_token<T, OP>(a, t, z.p);
       r.z = k.z;
       r.state = k.state;
+      r.id = k.id;
     }
     if (lane == 0) {
       s_token = k;
@@ -547,7 +611,7 @@ __global__ void __launch_bounds__(512) vocab_row_kernel(const VocabLossArgs a) {
     }
     return;
   }
-  float mx = -INFINITY, sum = 0.f;
+  float mx = -INFINITY, rest = 0.f;
   for (int j = threadIdx.x; j < z.nv; j += blockDim.x) {
     float o[N];
     Elem<T>::unpack(z.load(j), o);
@@ -558,16 +622,19 @@ __global__ void __launch_bounds__(512) vocab_row_kernel(const VocabLossArgs a) {
   for (int j = threadIdx.x; j < z.nv; j += blockDim.x) {
     float o[N];
     Elem<T>::unpack(z.load(j), o);
+    const int64_t own = (int64_t)k.id - z.first(j);
 #pragma unroll
-    for (int i = 0; i < N; ++i) sum += x(o[i]);
+    for (int i = 0; i < N; ++i) rest += i == own ? 0.f : ex2(x.arg(o[i]) - kShift);
   }
-  sum = block_sum(sum, red);
+  rest = block_sum(rest, red) * kShiftUp;
+  if (x.m == -INFINITY) rest = __int_as_float(0x7fffffff);  // no finite logit: no softmax
   if (threadIdx.x == 0) {
     rec->m = x.m;
-    rec->sum = sum;
+    rec->rest = rest;
   }
   if (!a.grad) return;
-  const float A = row_factor<OP>(a, k, x, sum, loss_factor(a)), As = A / sum;
+  const float A = row_factor<OP>(a, k, x.m, rest, loss_factor(a));
+  const float As = A / (k.id >= 0 ? rest + x(k.z) : rest);
   for (int j = threadIdx.x; j < z.nv; j += blockDim.x) {
     float o[N];
     Elem<T>::unpack(z.load(j), o);
@@ -580,7 +647,7 @@ __global__ void __launch_bounds__(512) vocab_row_kernel(const VocabLossArgs a) {
     for (int i = threadIdx.x; i < a.K; i += blockDim.x)
       if (s.id[i] >= 0) g.p[s.id[i]] = Elem<T>::t(As * x(s.z[i]) - A * weight_of(s, s.id[i]));
   } else {
-    if (threadIdx.x == 0) g.p[k.id] = Elem<T>::t(As * x(k.z) - A);
+    if (threadIdx.x == 0) g.p[k.id] = Elem<T>::t(-As * rest);  // A (q - 1)
   }
 }
 
@@ -631,21 +698,22 @@ struct StreamShared {
   uint64_t pairs_full[2], factor_full[2];
   uint4 edge[kTokens][2];  // a row's first and last vector, where they are partial
   Token token[kTokens];
-  float factor[2][4];  // A, A / sum, reference
+  float factor[2][4];  // A, A / sum, reference, sum without the token
   float2 pairs[2][kMaxCluster * kMaxConsumers];
   int abort;
 };
 
-// The row's reference and sum from all warps' pairs (one warp; the same bits in each).
-__device__ __forceinline__ void join_pairs(const float2* pairs, int n, C2 c2, int lane, float* m, float* sum) {
-  float mx = -INFINITY, v = 0.f;
+// The row's reference and the sum of all warps' pairs (one warp; the same bits in each). z: the
+// logit of the token that the pairs leave out (none: -infinity).
+__device__ __forceinline__ void join_pairs(const float2* pairs, int n, C2 c2, float z, int lane, float* m, float* rest) {
+  float mx = z, v = 0.f;
   for (int i = lane; i < n; i += 32) mx = fmaxf(mx, pairs[i].x);
   mx = warp_max(mx);
   const Expo x(c2, mx);
   for (int i = lane; i < n; i += 32) v += x.join(pairs[i].x, pairs[i].y);
   v = warp_sum(v);
   // a row without a finite logit has no softmax
-  *sum = mx == -INFINITY ? __int_as_float(0x7fffffff) : v;
+  *rest = mx == -INFINITY ? __int_as_float(0x7fffffff) : v;
   *m = mx;
 }
 
@@ -770,11 +838,14 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
         __syncwarp();
         if (lane == 0) {
           sh.token[e].state = state;
+          sh.token[e].id = r.id;
+          sh.token[e].z = r.z;
           if (rank == 0) {  // not the consumer's half
             recs[t].base = r.base;
             recs[t].z = r.z;
             recs[t].weight = r.weight;
             recs[t].state = state;
+            recs[t].id = r.id;
           }
           mbar_arrive(&sh.ent_full[e]);
         }
@@ -803,6 +874,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
           if (rank == 0) {
             recs[t].z = k.z;
             recs[t].state = k.state;
+            recs[t].id = k.id;
           }
           mbar_arrive(&sh.ent_full[e]);
         }
@@ -821,21 +893,24 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
         if (C > 1 && lane == 0) mbar_arrive_expect_tx(&sh.pairs_full[x & 1], (uint32_t)(C * CW) * 8u);
         __syncwarp();
         if (!wait_exchange(&sh.pairs_full[x & 1], x >> 1)) break;
-        float sum;
-        join_pairs(sh.pairs[x & 1], C * CW, C2{a.c2, a.c2_hi, a.c2_lo}, lane, &m, &sum);
+        const C2 c2 = {a.c2, a.c2_hi, a.c2_lo};
+        const bool apart = token.id >= 0;
+        float rest;
+        join_pairs(sh.pairs[x & 1], C * CW, c2, apart ? token.z : -INFINITY, lane, &m, &rest);
         if (a.grad) {
-          A = row_factor<OP>(a, token, Expo(C2{a.c2, a.c2_hi, a.c2_lo}, m), sum, factor);
-          As = A / sum;
+          A = row_factor<OP>(a, token, m, rest, factor);
+          As = A / (apart ? rest + Expo(c2, m)(token.z) : rest);
         }
         if (lane == 0) {
           sh.factor[x & 1][0] = A;
           sh.factor[x & 1][1] = As;
           sh.factor[x & 1][2] = m;
+          sh.factor[x & 1][3] = rest;
           mbar_arrive(&sh.factor_full[x & 1]);
           if (rank == 0) {
             RowRecord* rec = reinterpret_cast<RowRecord*>(a.records) + t;
             rec->m = m;
-            rec->sum = sum;
+            rec->rest = rest;
           }
         }
         ++x;
@@ -881,6 +956,9 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
     // the row that is summed: done of np pieces
     int t = cluster, np = 0, done = 0, part_n = 0;
     bool open = false;
+    // the token that the sum leaves out: its piece (-1: none in this block's part), and its
+    // element within the part where it is this thread's
+    int apart_piece = -1, apart = -1;
     float ref = -INFINITY, sum = 0.f;
     F2 nR2 = f2(0.f, 0.f);
     // the row that waits for its factor
@@ -903,6 +981,11 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
           done = 0;
           ref = -INFINITY;
           sum = 0.f;
+          const int id = sh.token[e].id;
+          const int own = (int)(((int64_t)id + z.a) / N) - j0;
+          const bool here = id >= 0 && own >= 0 && own < part_n;
+          apart_piece = here ? own / kPieceVecs : -1;
+          apart = here && own % Cfg::Lanes == tid ? (int)((int64_t)id + z.a - (int64_t)j0 * N) : -1;
           break;
         }
         if (a.grad) {
@@ -916,9 +999,8 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
         t += clusters;
       }
       if (open) {
-        // Sum against a reference that is the maximum of the thread's first vectors: the sum
-        // may grow to 2^40 before the reference is moved, which costs fp32 nothing, so the
-        // usual vector takes no maximum.
+        // Sum against a reference that is the maximum of the warp's first vectors: the usual
+        // vector takes no maximum, and the reference rarely moves.
         const int stop = tg >= 0 ? min(np, done + kAhead) : np;
         auto there = [&](int sl, int tn) {  // a row's gradient is owed: do not wait
           return __all_sync(0xffffffffu, mbar_test_wait(&sh.full[sl], (uint32_t)tn)) != 0;
@@ -938,11 +1020,19 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
           return sum + (ax + ay);
         };
         auto add_carefully = [&](const uint4* piece, int n, bool first) {
-          const float2 r = careful_sum<T>(piece, n, Cfg::Lanes, c2, first ? -INFINITY : ref, sum * kShiftUp);
+          const float2 r = careful_sum<T>(piece, n, Cfg::Lanes, c2, first ? -INFINITY : ref, sum);
           ref = r.x;
-          sum = r.y * kShiftDown;
+          sum = r.y;
           const float R = reference(ref, c2);
           nR2 = f2(R, R);
+        };
+        // the gradient writes this element by itself
+        auto leave_out = [&](int sl) {
+          if (apart >= 0) {
+            const int at = apart - apart_piece * (kPieceVecs * N);
+            blank<T>(reinterpret_cast<uint4*>(ring + (size_t)sl * kPieceBytes) + at / N, at % N);
+            fence_proxy_async_smem();  // before a later bulk copy into the slot
+          }
         };
         auto next_slot = [&] {
           if (!a.grad) {
@@ -973,6 +1063,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
               goto out;
             }
             const uint4* piece1 = piece_at(slot1);
+            if ((unsigned)(apart_piece - done) < 2u) leave_out(apart_piece == done ? slot : slot1);
             uint4 raw[2 * Cfg::VPT];
 #pragma unroll
             for (int v = 0; v < Cfg::VPT; ++v) {
@@ -983,7 +1074,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
 #pragma unroll
             for (int v = 0; v < 2 * Cfg::VPT; ++v) add_vec(raw[v], acc);
             const float s1 = total(acc);
-            if (s1 <= 1.0995e12f) {
+            if (s1 <= kMostSum) {
               sum = s1;
             } else {  // NaN too
               add_carefully(piece, Cfg::VPT, false);
@@ -995,6 +1086,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
             continue;
           }
           const int left = (end - tid + Cfg::Lanes - 1) / Cfg::Lanes;  // this thread's vectors (or < 1)
+          if (apart_piece == done) leave_out(slot);
           uint4 raw[Cfg::VPT];
           if (end >= kPieceVecs) {
 #pragma unroll
@@ -1006,6 +1098,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
           if (done == 0) {
 #pragma unroll
             for (int v = 0; v < Cfg::VPT; ++v) ref = max_of<T>(raw[v], ref);
+            ref = warp_max(ref);
             const float R = reference(ref, c2);
             nR2 = f2(R, R);
           }
@@ -1016,7 +1109,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
             add_vec(raw[v], acc);
           }
           const float s1 = total(acc);
-          if (s1 <= 1.0995e12f) sum = s1;
+          if (s1 <= kMostSum) sum = s1;
           else if (left > 0) add_carefully(piece, min(left, Cfg::VPT), done == 0);  // NaN too
           ++done;
           next_slot();
@@ -1092,7 +1185,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
           const Token token = sh.token[eg];
           const int own = (int)(((int64_t)token.id + z.a) / N) - j0;
           if (own >= 0 && own < j1 - j0 && own % Cfg::Lanes == tid)
-            g.p[token.id] = Elem<T>::t(As * w(token.z) - sh.factor[xg & 1][0]);
+            g.p[token.id] = Elem<T>::t(-As * sh.factor[xg & 1][3]);  // A (q - 1)
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(OP == kOpDistill ? &sh.dense_done[eg] : &sh.ent_done[eg]);
@@ -1144,8 +1237,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
 
 // Outputs of all rows from their records, one thread per row, and the loss as the sum over
 // rows in 64 bits: blocks leave partial sums, the last one adds them in their order, so the
-// loss has the same bits on every run. Log-probabilities are formed in 64 bits: in fp32 the
-// rounding of ln(sum) near 12 alone is 5e-7, and a sequence's log-ratio sums hundreds.
+// loss has the same bits on every run.
 constexpr int kFinishThreads = 256;
 template <int OP>
 __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const VocabLossArgs a) {
@@ -1153,15 +1245,12 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Voca
   __shared__ bool last;
   const int t = blockIdx.x * kFinishThreads + threadIdx.x;
   const float nan = __int_as_float(0x7fffffff);
-  const double ln2 = 0.69314718055994530942;
   float loss = 0.f;
   if (t < a.T) {
     const RowRecord r = reinterpret_cast<const RowRecord*>(a.records)[t];
-    const Expo x(C2{a.c2, a.c2_hi, a.c2_lo}, r.m);
+    const C2 c2 = {a.c2, a.c2_hi, a.c2_lo};
     double lp = 0.0;  // ln q of the token (of the entry that zref is from)
-    if (r.state == kRowOn)
-      lp = (x.far ? ((double)r.z - (double)r.m) / a.tau64 : (double)r.z / a.tau64 - (double)x.M2 * ln2) -
-           log((double)r.sum) + kExpMeanError;
+    if (r.state == kRowOn) lp = row_logp(c2, r.z, r.m, r.rest, r.id >= 0);
     if constexpr (OP == kOpDistill) {
       if (r.state == kRowOn) loss = (float)((double)a.tau * a.tau * (r.base - (double)r.weight * lp));
       else if (r.state == kRowBad) loss = nan;
@@ -1170,15 +1259,19 @@ __global__ void __launch_bounds__(kFinishThreads) vocab_finish_kernel(const Voca
       if (r.state == kRowBad) lp = (double)nan;
       a.logp[t] = (float)lp;
       if constexpr (OP == kOpLogp) {
-        if (a.lse) reinterpret_cast<float2*>(a.lse)[t] = on ? make_float2(r.m, r.sum) : make_float2(0.f, 0.f);
+        if (a.lse) {
+          reinterpret_cast<float2*>(a.lse)[t] = on ? make_float2(r.m, r.rest + Expo(c2, r.m)(r.z)) : make_float2(0.f, 0.f);
+          a.rest[t] = on ? r.rest : 0.f;
+        }
         if (a.ratio) {
           a.ratio[t] = on ? (float)(lp - (double)a.ref_logp[t]) : 0.f;
           a.row_coef[t] = 0.f;  // rows of no pair keep it
         }
       } else {
         PolicyTerm o = {0.f, 0.f, 0.f};
+        const double quick = r.state == kRowOn ? quick_logp(c2, r.z, r.m, r.rest) : lp;
         if (on)
-          o = policy_term(a, a.adv[t], expf((float)(lp - (double)a.old_logp[t])),
+          o = policy_term(a, a.adv[t], expf((float)(quick - (double)a.old_logp[t])),
                           a.ref_logp ? (float)((double)a.ref_logp[t] - lp) : 0.f, a.ref_logp != nullptr);
         loss = o.loss;
         a.kl[t] = o.kl;
@@ -1372,7 +1465,7 @@ __global__ void __launch_bounds__(kGradThreads) preference_grad_kernel(const Voc
   if (label < a.V) {
     const int own = (int)((label + z.a) / N) - j0;
     if (own >= 0 && own < j1 - j0 && own % kGradThreads == tid)
-      g.p[label] = Elem<T>::t(As * x(Elem<T>::f(z.p[label])) - A);
+      g.p[label] = Elem<T>::t(-As * a.rest[t]);  // A (q - 1)
   }
 }
 

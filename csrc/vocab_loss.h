@@ -51,7 +51,8 @@ struct VocabLossArgs {
   float* kl = nullptr;    // [T], kOpPolicy
   float* ratio = nullptr;  // [T], kOpLogp: logp - ref_logp, 0 for rows not in the loss (optional)
   float* row_coef = nullptr;  // [T], kOpLogp with ratio: set to 0
-  float* lse = nullptr;    // [T, 2], kOpLogp: a reference m of the row and its sum of 2^((z - m) c2) (optional)
+  float* lse = nullptr;    // [T, 2], kOpLogp: a reference m of the row and its sum of 2^((z - m) c2) (optional) ...
+  float* rest = nullptr;   // [T], with lse: the sum without the label's term
 };
 constexpr int kRowRecordBytes = 32;
 int vocab_finish_blocks(int T);
