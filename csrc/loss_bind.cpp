@@ -405,10 +405,22 @@ at::Tensor once(AutogradContext* ctx, const at::Tensor& g) {
 // A loss whose forward has formed the gradient in its pass over the logits. It is handed out
 // once, scaled in place (not touched where the upstream gradient is 1). A second backward
 // through the same graph, and fp16 logits, whose unscaled gradient could leave the type's
-// range, compute it from the logits.
+// range, compute it from the logits. So does a backward that is captured apart from its forward:
+// every replay would scale the kept gradient again.
 bool formed_in_forward(const at::Tensor& z) { return z.scalar_type() != at::kHalf; }
+// The capture that the current stream is in, 0 for none.
+int64_t capture_id() {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(cs(), &status, &id));
+  return status == cudaStreamCaptureStatusActive ? (int64_t)id : 0;
+}
 // Keeps a buffer for the gradient and returns its view.
 at::Tensor keep_gradient(AutogradContext* ctx, const at::Tensor& z) {
+  if (z.is_cuda()) {  // others are refused with the checks of the call
+    const c10::cuda::CUDAGuard guard(z.device());
+    ctx->saved_data["capture"] = capture_id();
+  }
   const at::Tensor flat = gradient_storage(z), g = gradient_view(flat, z);
   ctx->saved_data["grad"] = flat;
   if (flat.dim() != 2)
@@ -417,7 +429,7 @@ at::Tensor keep_gradient(AutogradContext* ctx, const at::Tensor& z) {
 }
 at::Tensor take_formed(AutogradContext* ctx, const at::Tensor& up) {
   auto& kept = ctx->saved_data["grad"];
-  if (!kept.isTensor()) return {};
+  if (!kept.isTensor() || ctx->saved_data["capture"].toInt() != capture_id()) return {};
   at::Tensor flat = kept.toTensor();
   kept = c10::IValue();
   scale_grad(flat, up);  // with what lies between the rows, which nothing reads
