@@ -583,6 +583,7 @@ void register_losses(pybind11::module& m) {
   m.def("distill_loss", &distill_loss);
   m.def("policy_loss", &policy_loss);
   m.def("preference_fwd", &preference_fwd);
+  m.def("scale_grad", &scale_grad);
   m.def("router_balance_fwd", &router_balance_fwd);
   m.def("router_balance_bwd", &router_balance_bwd);
 }

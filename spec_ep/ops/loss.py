@@ -191,7 +191,10 @@ class _LMHead(torch.autograd.Function):
         dh = dense_dgrad(dlogits, w) if ctx.needs_input_grad[0] else None
         if row_scale is None:
             dw = dense_wgrad(dlogits, h) if ctx.needs_input_grad[1] else None
-            return None if dh is None else dh * up.to(h.dtype), None if dw is None else dw * up.to(w.dtype), None
+            for g in (dh, dw):
+                if g is not None:
+                    load().scale_grad(g, up)  # in place, by the fp32 factor; untouched where it is 1
+            return dh, dw, None
         # the rows' factors go to the small side of each product: onto dh, and onto h, where
         # they cost one more rounding to bf16 (2^-9 of each term of a sum over tokens)
         s = (row_scale * up)[:, None]
