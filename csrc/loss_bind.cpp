@@ -392,7 +392,11 @@ at::Tensor router_balance_bwd(const at::Tensor& x, const at::Tensor& topk_e, con
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-bool wants_grad(const at::Tensor& z) { return at::GradMode::is_enabled() && z.requires_grad(); }
+// Also a forward-mode tangent takes the way through autograd, which refuses it: the kernels
+// alone would drop it.
+bool wants_grad(const at::Tensor& z) {
+  return (at::GradMode::is_enabled() && z.requires_grad()) || z._fw_grad(/*level=*/0).defined();
+}
 
 // Gradients here are not themselves differentiable: whoever tries, through the logits that
 // they depend on, gets an error.

@@ -19,6 +19,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+import torch.autograd.forward_ad as fwd
 from torch.autograd.function import once_differentiable
 
 from ._ext import load
@@ -202,8 +203,13 @@ class _LMHead(torch.autograd.Function):
         return None if dh is None else (dh * s).to(h.dtype), dw, None
 
 
+def _has_tangent(*ts):
+    return fwd._current_level >= 0 and any(fwd.unpack_dual(t).tangent is not None for t in ts)
+
+
 def _lm_head(h, w, kernel):
-    if torch.is_grad_enabled() and (h.requires_grad or w.requires_grad):
+    # a forward-mode tangent too goes through autograd, which refuses it
+    if (torch.is_grad_enabled() and (h.requires_grad or w.requires_grad)) or _has_tangent(h, w):
         return _LMHead.apply(h, w, kernel)
     loss, _, *aux = kernel(dense_fwd(h, w), None)
     return (loss, *aux)
