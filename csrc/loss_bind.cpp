@@ -6,6 +6,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <cmath>
 #include <string>
 
@@ -46,6 +47,16 @@ bool ids_are_64(const at::Tensor& t, const char* name) {
   return t.scalar_type() == at::kLong;
 }
 
+// Limits of the waits in the calls to come (test_stall).
+std::atomic<int64_t> g_wait_ns{2000000000}, g_stall_row{-1};
+
+// Makes the waits for a row run out after wait_ns in every call until test_stall(-1, 0).
+void test_stall(int64_t row, int64_t wait_ns) {
+  TORCH_CHECK(row >= -1 && row < 0x7fffffff && wait_ns >= 0 && wait_ns <= 2000000000, "a row and at most 2 s");
+  g_stall_row = row;
+  g_wait_ns = wait_ns > 0 ? wait_ns : 2000000000;
+}
+
 // Common part: logits, gradient buffer and temperature.
 sepx::VocabLossArgs vocab_args(const at::Tensor& z, const c10::optional<at::Tensor>& grad, double tau) {
   TORCH_CHECK(z.dim() == 2, "logits must be [T, V]");
@@ -54,6 +65,8 @@ sepx::VocabLossArgs vocab_args(const at::Tensor& z, const c10::optional<at::Tens
   TORCH_CHECK(z.stride(1) == 1 || z.size(1) == 1, "logits must have unit stride along the vocabulary");
   TORCH_CHECK(std::isfinite(tau) && tau > 0, "temperature must be positive and finite");
   sepx::VocabLossArgs a;
+  a.wait_ns = (uint64_t)g_wait_ns.load();
+  a.stall_row = (int)g_stall_row.load();
   a.z = z.data_ptr();
   a.z_stride = z.stride(0);
   a.dtype = vocab_dtype(z, "logits");
@@ -588,6 +601,7 @@ void register_losses(pybind11::module& m) {
   m.def("policy_loss", &policy_loss);
   m.def("preference_fwd", &preference_fwd);
   m.def("scale_grad", &scale_grad);
+  m.def("test_stall", &test_stall, "tests: the waits for this row of the vocabulary losses run out");
   m.def("router_balance_fwd", &router_balance_fwd);
   m.def("router_balance_bwd", &router_balance_bwd);
 }

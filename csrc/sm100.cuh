@@ -326,6 +326,9 @@ __device__ __forceinline__ uint32_t mapa_shared(uint32_t a, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void st_cluster_u32(uint32_t to, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(v) : "memory");
+}
 // Two floats to a shared::cluster address, counted (8 bytes) on the mbarrier at the
 // shared::cluster address `bar` of the same CTA.
 __device__ __forceinline__ void st_async_f2(uint32_t to, float a, float b, uint32_t bar) {

@@ -340,7 +340,7 @@ __device__ __noinline__ void careful_store(const uint4* v, T* row, int V, int64_
 // Bounded waits, out of line. The usual one sleeps in the barrier (polls of a waiting warp take
 // issue slots from the working ones); the exchange of a row's sums, where every cycle
 // counts, polls.
-__device__ __noinline__ bool wait_asleep(uint64_t* bar, uint32_t parity, volatile int* abort) {
+__device__ __noinline__ bool wait_asleep(uint64_t* bar, uint32_t parity, volatile int* abort, uint64_t limit_ns) {
   const uint64_t t0 = globaltimer_ns();
   for (;;) {
     uint32_t ok;
@@ -353,14 +353,14 @@ __device__ __noinline__ bool wait_asleep(uint64_t* bar, uint32_t parity, volatil
         : "memory");
     if (ok) return true;
     if (*abort) return false;
-    if (globaltimer_ns() - t0 > 2000000000ull) {
+    if (globaltimer_ns() - t0 > limit_ns) {
       *abort = 1;
       return false;
     }
   }
 }
-__device__ __noinline__ bool wait_awake(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  return mbar_wait_bounded(bar, parity, abort, nullptr, 2000000000ull);
+__device__ __noinline__ bool wait_awake(uint64_t* bar, uint32_t parity, volatile int* abort, uint64_t limit_ns) {
+  return mbar_wait_bounded(bar, parity, abort, nullptr, limit_ns);
 }
 
 // ------------------------------------------------------------------------------------
@@ -667,7 +667,8 @@ __global__ void __launch_bounds__(512) vocab_row_kernel(const VocabLossArgs a) {
 // Partial sums travel as (reference, sum) pairs of each warp, with asynchronous stores that
 // complete on the receiver's mbarrier. Pair buffers alternate: a warp sends row r + 2 after it
 // has row r + 1 of every warp, and each of those left after its block had all of row r.
-// Every wait is bounded; one that runs out turns the call's outputs into NaN.
+// Every wait is bounded; one that runs out turns the outputs of all the cluster's rows,
+// gradients among them, and with them the loss, into NaN.
 //
 // What bounds it: memory would take 380 us for 4096 x 151936 bf16 with gradients (2.5 GB at
 // 6.55 TB/s); measured 484-502 us, 5.1 TB/s, with every byte moved once (a capture of 1024
@@ -755,12 +756,12 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
   auto wait = [&](uint64_t* bar, int phase) {
     const uint32_t parity = (uint32_t)phase & 1u;
     return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) ||
-           __all_sync(0xffffffffu, wait_asleep(bar, parity, abort));
+           __all_sync(0xffffffffu, wait_asleep(bar, parity, abort, a.wait_ns));
   };
   auto wait_exchange = [&](uint64_t* bar, int phase) {
     const uint32_t parity = (uint32_t)phase & 1u;
     return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) ||
-           __all_sync(0xffffffffu, wait_awake(bar, parity, abort));
+           __all_sync(0xffffffffu, wait_awake(bar, parity, abort, a.wait_ns));
   };
   const int log2c = 31 - __clz(C);
   // this block's vectors of row t
@@ -826,6 +827,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
       int e = 0, lap = 0;
       for (int t = cluster; t < a.T; t += clusters) {
         const RowVec<T> z = row_z(t);
+        if (t == a.stall_row && rank == 0) break;
         if (!wait(&sh.ent_done[e], lap ^ 1)) break;
         const bool head = !z.full(0), tail = !z.full(z.nv - 1);
         if (head || tail) {  // lanes 0..N-1: the first vector, 16..16+N-1: the last
@@ -861,9 +863,9 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
         if (!__any_sync(0xffffffffu, mine)) break;
         const int e = (g0 + lane) % kTokens;
         bool ok = true;
-        if (mine) ok = wait_asleep(&sh.ent_done[e], (uint32_t)(((g0 + lane) / kTokens) & 1) ^ 1u, abort);
+        if (mine) ok = wait_asleep(&sh.ent_done[e], (uint32_t)(((g0 + lane) / kTokens) & 1) ^ 1u, abort, a.wait_ns);
         if (!__all_sync(0xffffffffu, ok)) break;
-        if (mine) {
+        if (mine && !(t == a.stall_row && rank == 0)) {
           const RowVec<T> z = row_z((int)t);
           const Token k = load_token<T, OP>(a, (int)t, z.p);
           if (k.state != kRowOff) {
@@ -1222,16 +1224,29 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
     }
   out:;
   }
-  if (*abort) {  // copies in flight land long before this
-    const uint64_t t0 = globaltimer_ns();
+  __syncthreads();
+  if (C > 1) {
+    // a row is lost to all blocks of the cluster where one has given up
+    if (*abort && threadIdx.x < (unsigned)C) st_cluster_u32(mapa_shared(smem_u32(&sh.abort), threadIdx.x), 1u);
+    cluster_sync();  // no block leaves while another may still write to it
+  }
+  if (*abort) {
+    const uint64_t t0 = globaltimer_ns();  // copies and pairs in flight land long before this
     while (globaltimer_ns() - t0 < 1000000) {
     }
-  }
-  __syncthreads();
-  if (C > 1) cluster_sync();  // no block leaves while another may still write to it
-  if (*abort && threadIdx.x == 0) {
     RowRecord* recs = reinterpret_cast<RowRecord*>(a.records);
-    for (int t = cluster; t < a.T; t += clusters) recs[t].state = kRowBad;
+    float o[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = __int_as_float(0x7fffffff);
+    for (int t = cluster; t < a.T; t += clusters) {
+      if (threadIdx.x == 0) recs[t].state = kRowBad;
+      if (a.grad) {  // what it holds may be the logits, or nothing yet
+        const RowVec<T> z = row_z(t), g(reinterpret_cast<T*>(a.grad) + (int64_t)t * a.grad_stride, a.V);
+        int j0, j1;
+        part(z, &j0, &j1);
+        for (int j = j0 + (int)threadIdx.x; j < j1; j += Cfg::Threads) g.store(z.first(j), o);
+      }
+    }
   }
 }
 

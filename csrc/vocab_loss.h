@@ -41,6 +41,10 @@ struct VocabLossArgs {
   float clip_low = 0.f, clip_high = 0.f, kl_coef = 0.f;
   const int* offsets = nullptr;  // kOpLogp: rows outside [offsets[0], offsets[num_seq]) are not in the loss
   int num_seq = 0;
+  // How long a wait between warps or blocks may last, and a row (-1: none) that is never
+  // announced to those who wait for it: a test makes the waits run out.
+  uint64_t wait_ns = 2000000000;
+  int stall_row = -1;
   // scratch
   void* records = nullptr;     // [T] records of kRowRecordBytes each
   double* partial = nullptr;   // [vocab_finish_blocks(T)]
