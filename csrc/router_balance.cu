@@ -61,7 +61,8 @@ __device__ __forceinline__ float warp_max(float v) {  // NaN gives way
 }
 
 // Order of floats as unsigned numbers (NaN above everything, -0 equal to +0); 0 is below
-// every value and marks what is taken or outside the row.
+// every value and marks what is taken or outside the row. The addition turns -0 into +0, and
+// any NaN, of either sign, into the one positive NaN that fp32 arithmetic returns.
 __device__ __forceinline__ uint32_t order_key(float v) {
   const uint32_t u = __float_as_uint(v + 0.f);
   const uint32_t k = u ^ ((u & 0x80000000u) ? 0xffffffffu : 0x80000000u);
