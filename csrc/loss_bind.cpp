@@ -602,6 +602,4 @@ void register_losses(pybind11::module& m) {
   m.def("preference_fwd", &preference_fwd);
   m.def("scale_grad", &scale_grad);
   m.def("test_stall", &test_stall, "tests: the waits for this row of the vocabulary losses run out");
-  m.def("router_balance_fwd", &router_balance_fwd);
-  m.def("router_balance_bwd", &router_balance_bwd);
 }
