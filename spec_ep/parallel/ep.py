@@ -430,7 +430,8 @@ class _EPMoE(torch.autograd.Function):
         del dxp
         # The expert weight gradients (and their optimizer updates) feed nothing downstream,
         # so they run while the other ranks' partials of this layer are still in flight.
-        fused = getattr(sink, "fused_wgrad", None) if sink is not None else None
+        fused_for = getattr(sink, "fused_for", None)
+        fused = fused_for(w_gu) if fused_for is not None else None
         g_gu = g_d = None
         with stage("ep.expert_wgrad"):
             if fused is not None:  # optimizer applied inside the wgrad GEMM epilogue
@@ -462,4 +463,8 @@ def ep_moe(x, topk_e, topk_w, w_gu, w_d, ep: ExpertParallel, grad_sink=None, res
     optionally gives per-call ``(e2r, e2l)`` device tables (speculative replicas)
     instead of the communicator's placement.
     """
+    used = getattr(grad_sink, "used", None)
+    if used is not None and torch.is_grad_enabled() and w_gu.requires_grad:
+        used(w_gu)
+        used(w_d)
     return _EPMoE.apply(x, topk_w, w_gu, w_d, topk_e, ep, grad_sink, residual, route)

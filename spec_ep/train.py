@@ -72,14 +72,16 @@ class Trainer:
         wait between layers). If some layer's rows outgrew its budget on any rank, the
         forward is discarded (nothing was updated yet) and run again with the grown
         budgets; the first step learns the budgets with exact sizes."""
-        ep = getattr(self.model, "ep", None)
-        if ep is None or not hasattr(ep, "run_pass"):
-            return loss_fn()
         calls = [0]
 
         def fwd():
             calls[0] += 1
+            self.expert_updater.begin()
             return loss_fn()
+
+        ep = getattr(self.model, "ep", None)
+        if ep is None or not hasattr(ep, "run_pass"):
+            return fwd()
 
         loss = ep.run_pass(fwd)
         self.budget_retries += calls[0] - 1
@@ -90,14 +92,19 @@ class Trainer:
         return self.step(lambda: self.model(input_ids, labels, num_valid))
 
     def step(self, loss_fn):
-        """One optimizer step on ``loss_fn()``, a scalar loss of the model (one forward of
-        it, which may run again when row budgets were outgrown): for instance
-        ``trainer.step(lambda: model.policy(ids, actions, old, adv).loss)``."""
+        """One optimizer step on ``loss_fn()``, a scalar loss of the model (which may run
+        again when row budgets were outgrown): for instance
+        ``trainer.step(lambda: model.policy(ids, actions, old, adv).loss)``. With several
+        forwards of the model in it the experts' gradients (fp32) are kept until the last
+        forward's backward has used their weights; with one they are applied at once."""
         if self.buckets is not None:
             self.buckets.begin()
-        loss = self._forward(loss_fn)
-        loss.backward()
-        self.expert_updater.flush()
+        try:
+            loss = self._forward(loss_fn)
+            loss.backward()
+            self.expert_updater.flush()
+        finally:
+            self.expert_updater.end()
         self._sync_dense_grads()
         self.opt.step()
         return loss.detach()
@@ -235,6 +242,12 @@ class _ExpertUpdater:
     faster than the two-kernel path on the Qwen3-30B-A3B shapes. Otherwise (fp32 state,
     or replicas that need an all-reduce of the gradient first) the GEMM writes an fp32
     gradient and the streaming optimizer kernel applies it.
+
+    Both update the weights while the backward runs. That is right for a step of one forward:
+    nothing uses a layer's expert weights after their gradient. In a step of several (``used``
+    counts them between ``begin`` and ``end``), other forwards' backwards still do, so the
+    gradients are summed and the last one applies the sum; ``flush`` applies what a forward
+    that took no part in the loss left waiting.
     """
 
     # gradients whose expert-DP all-reduce may still be in flight: one layer's two
@@ -249,8 +262,39 @@ class _ExpertUpdater:
         use = trainer.fuse_expert_optimizer and trainer.expert_world == 1 and not self.rep_slots
         self.fused_wgrad = trainer.opt.fused_wgrad if use else None
         self.pending = []  # (param, grad, work) with the expert-DP all-reduce in flight
+        self.end()
+
+    def begin(self):
+        """A step's loss is about to be computed (again, where a pass is run again)."""
+        self.in_step = True
+        self.uses = {}  # id(param): forwards that used it
+        self.left = {}  # id(param): of those, the ones whose gradient is still to come
+        self.sums = {}  # id(param): (param, sum of the gradients so far)
+
+    def end(self):
+        self.begin()
+        self.in_step = False
+
+    def used(self, p):
+        """A forward with gradients has used ``p``."""
+        if self.in_step:
+            self.uses[id(p)] = self.left[id(p)] = self.uses.get(id(p), 0) + 1
+
+    def fused_for(self, p):
+        """The update inside the weight-gradient GEMM, where ``p`` may take it now."""
+        return self.fused_wgrad if self.uses.get(id(p), 0) <= 1 else None
 
     def __call__(self, p, g):
+        if self.uses.get(id(p), 0) > 1:
+            if id(p) in self.sums:
+                g = self.sums.pop(id(p))[1].add_(g)
+            self.left[id(p)] -= 1
+            if self.left[id(p)] > 0:
+                self.sums[id(p)] = (p, g)
+                return
+        self._reduce(p, g)
+
+    def _reduce(self, p, g):
         t = self.t
         if self.rep_slots:
             sum_replica_grads(g, self.rep_slots, self.ep_group)
@@ -269,6 +313,9 @@ class _ExpertUpdater:
         self.t.opt.apply_now(p, g)
 
     def flush(self):
-        """Apply every update still waiting for its all-reduce (end of the backward)."""
+        """Apply every update still waiting (end of the backward)."""
+        for p, g in self.sums.values():
+            self._reduce(p, g)
+        self.sums = {}
         while self.pending:
             self._apply(*self.pending.pop(0))
