@@ -63,7 +63,7 @@ class Qwen3MoeLayer(nn.Module):
         self.router_logit_bias = None  # optional fp32 [E] bias added to the router logits (skew studies)
         self.routing_callback = None  # receives topk expert ids (routing capture)
         self.spec = None  # SpeculativeExperts (speculative replication, inference only)
-        self.balance = False  # training: route with the balance loss, into the two below
+        self.balance = False  # route with the balance loss, into the two below
         self.balance_loss = None  # this forward's loss, until the model has added it to its own
         self.expert_counts = None  # tokens of the last forward that chose each expert, [E] int32
 
@@ -89,9 +89,10 @@ class Qwen3MoeLayer(nn.Module):
         logits = linear(h, self.w_router)
         if self.router_logit_bias is not None:
             logits = logits.float() + self.router_logit_bias
-        if self.balance and torch.is_grad_enabled():
-            topk_w, topk_e, self.balance_loss, self.expert_counts = router_topk_balanced(
+        if self.balance:  # without gradients too: a rollout routes with the training pass's bits
+            topk_w, topk_e, loss, self.expert_counts = router_topk_balanced(
                 logits, cfg.top_k, cfg.norm_topk_prob, self.router_bias)
+            self.balance_loss = loss if torch.is_grad_enabled() else None
         else:
             topk_w, topk_e = router_topk(logits.float(), cfg.top_k, cfg.norm_topk_prob, self.router_bias)
         if self.routing_callback is not None:
