@@ -27,8 +27,8 @@ import torch.nn.functional as F
 
 from ..ops.attention import causal_gqa_attention
 from ..ops.linear import dense_fwd, linear
-from ..ops.loss import (PolicyLoss, lm_head_distill, lm_head_policy, lm_head_token_logp,
-                        lm_head_xent)
+from ..ops.loss import (PolicyLoss, PreferenceLoss, lm_head_distill, lm_head_policy, lm_head_preference,
+                        lm_head_token_logp, lm_head_xent)
 from ..ops.norm import add_rms_norm, rms_norm, rms_norm_res
 from ..ops.rope import qk_norm_rope
 from ..ops.router import router_topk, router_topk_balanced
@@ -104,9 +104,9 @@ class Qwen3MoeLayer(nn.Module):
 
 
 class Qwen3MoeForCausalLM(nn.Module):
-    """Decoder-only MoE LM; ``forward(input_ids, labels)`` returns the mean CE loss, ``distill``
-    and ``policy`` the losses of their names. ``set_balance_loss`` adds the routers' balance
-    loss to each."""
+    """Decoder-only MoE LM; ``forward(input_ids, labels)`` returns the mean CE loss, ``distill``,
+    ``policy`` and ``preference`` the losses of their names. ``set_balance_loss`` adds the
+    routers' balance loss to each."""
 
     def __init__(self, cfg: MoEModelConfig, ep: ExpertParallel, device=None, dtype=torch.bfloat16):
         super().__init__()
@@ -133,47 +133,78 @@ class Qwen3MoeForCausalLM(nn.Module):
             layer.grad_sink = sink
 
     def set_balance_loss(self, coef: float):
-        """Add ``coef`` times the layers' mean router balance loss to every training loss
-        (0: off). Each layer then also keeps its last forward's ``expert_counts``."""
+        """Add ``coef`` times the layers' mean router balance loss to the losses that this model
+        returns (0: off); a loss formed from ``hidden_states`` gets none. Each layer then also
+        keeps its last forward's ``expert_counts``."""
         if not coef >= 0.0:
             raise ValueError(f"the balance loss's coefficient must be >= 0, not {coef}")
         self.balance_coef = float(coef)
         for layer in self.layers:
             layer.balance = coef > 0.0
 
-    def _with_balance(self, loss):
-        if self.balance_coef == 0.0 or not torch.is_grad_enabled():
-            return loss
-        parts = [layer.balance_loss for layer in self.layers]
-        for layer in self.layers:
-            layer.balance_loss = None  # its graph lives as long as the loss's
-        return loss + self.balance_coef * torch.stack(parts).mean()
-
-    def hidden_states(self, input_ids, pos=None):
+    def _hidden(self, input_ids, pos):
+        """Hidden states of one token stream, and the layers' balance losses (none without
+        gradients, or where the loss is off)."""
         x = F.embedding(input_ids.view(-1), self.embed)
+        balance = []
         for layer in self.layers:
             x = layer(x, pos)
-        return rms_norm(x, self.final_norm, self.cfg.rms_norm_eps)
+            if layer.balance_loss is not None:
+                balance.append(layer.balance_loss)
+                layer.balance_loss = None  # its graph lives as long as the loss's
+        return rms_norm(x, self.final_norm, self.cfg.rms_norm_eps), balance
+
+    def _with_balance(self, loss, balance):
+        return loss + self.balance_coef * torch.stack(balance).mean() if balance else loss
+
+    def hidden_states(self, input_ids, pos=None):
+        return self._hidden(input_ids, pos)[0]
 
     def forward(self, input_ids, labels=None, num_valid=None, pos=None):
-        h = self.hidden_states(input_ids, pos)
+        h, balance = self._hidden(input_ids, pos)
         if labels is None:
             return dense_fwd(h, self.lm_head)
-        return self._with_balance(lm_head_xent(h, self.lm_head, labels.view(-1), num_valid))
+        return self._with_balance(lm_head_xent(h, self.lm_head, labels.view(-1), num_valid), balance)
 
     def distill(self, input_ids, teacher_ids, teacher_logits, temperature=1.0, num_valid=None, pos=None):
         """Distillation loss of one token stream from a teacher's top logits ``[T, K]`` per
         token (see ``spec_ep.ops.loss.topk_distill_loss``)."""
-        h = self.hidden_states(input_ids, pos)
-        return self._with_balance(lm_head_distill(h, self.lm_head, teacher_ids, teacher_logits, temperature, num_valid))
+        h, balance = self._hidden(input_ids, pos)
+        return self._with_balance(lm_head_distill(h, self.lm_head, teacher_ids, teacher_logits, temperature, num_valid),
+                                  balance)
 
     def policy(self, input_ids, actions, old_logp, advantages, ref_logp=None, pos=None, **kw) -> PolicyLoss:
         """Clipped policy loss of one token stream: ``actions[t]`` is the token chosen after
         token ``t``, -1 where none was (see ``spec_ep.ops.loss.clipped_policy_loss``, whose
         other arguments go through ``kw``)."""
-        h = self.hidden_states(input_ids, pos)
+        h, balance = self._hidden(input_ids, pos)
         out = lm_head_policy(h, self.lm_head, actions.view(-1), old_logp, advantages, ref_logp, **kw)
-        return out._replace(loss=self._with_balance(out.loss))
+        return out._replace(loss=self._with_balance(out.loss, balance))
+
+    def preference(self, sequences, labels, ref_logp, beta=0.1, label_smoothing=0.0) -> PreferenceLoss:
+        """Paired preference loss of ``2 * pairs`` token sequences, the chosen one of each pair
+        before the rejected one, each through a forward of its own (attention is causal over a
+        whole token stream). ``labels[s]`` and ``ref_logp[s]`` belong to ``sequences[s]``: the
+        next tokens, -1 where not in the loss, and the reference model's ``token_logp`` of them
+        (see ``spec_ep.ops.loss.preference_loss``, which has the sequences one after another)."""
+        if not sequences or len(sequences) % 2:
+            raise ValueError(f"sequences must come in pairs, not {len(sequences)}")
+        if len(labels) != len(sequences) or len(ref_logp) != len(sequences):
+            raise ValueError("every sequence needs its labels and ref_logp")
+        ends = [0]
+        for s, y, r in zip(sequences, labels, ref_logp):
+            if not s.numel() == y.numel() == r.numel():
+                raise ValueError("a sequence, its labels and its ref_logp must have one length")
+            ends.append(ends[-1] + s.numel())
+        hs, balance = [], []
+        for s in sequences:
+            h, b = self._hidden(s, None)
+            hs.append(h)
+            balance += b
+        off = torch.tensor(ends, dtype=torch.int32, device=hs[0].device)
+        out = lm_head_preference(torch.cat(hs), self.lm_head, torch.cat([y.view(-1) for y in labels]), off,
+                                 torch.cat([r.view(-1) for r in ref_logp]), beta, label_smoothing)
+        return out._replace(loss=self._with_balance(out.loss, balance))
 
     @torch.no_grad()
     def token_logp(self, input_ids, labels, temperature=1.0, pos=None):
