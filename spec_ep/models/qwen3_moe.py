@@ -67,7 +67,7 @@ class Qwen3MoeLayer(nn.Module):
         self.balance_loss = None  # this forward's loss, until the model has added it to its own
         self.expert_counts = None  # tokens of the last forward that chose each expert, [E] int32
 
-    def forward(self, x, pos=None):
+    def forward(self, x, pos=None, valid=None):
         cfg = self.cfg
         spec = self.spec
         x_in = x
@@ -91,7 +91,7 @@ class Qwen3MoeLayer(nn.Module):
             logits = logits.float() + self.router_logit_bias
         if self.balance:  # without gradients too: a rollout routes with the training pass's bits
             topk_w, topk_e, loss, self.expert_counts = router_topk_balanced(
-                logits, cfg.top_k, cfg.norm_topk_prob, self.router_bias)
+                logits, cfg.top_k, cfg.norm_topk_prob, self.router_bias, valid)
             self.balance_loss = loss if torch.is_grad_enabled() else None
         else:
             topk_w, topk_e = router_topk(logits.float(), cfg.top_k, cfg.norm_topk_prob, self.router_bias)
@@ -134,21 +134,23 @@ class Qwen3MoeForCausalLM(nn.Module):
 
     def set_balance_loss(self, coef: float):
         """Add ``coef`` times the layers' mean router balance loss to the losses that this model
-        returns (0: off); a loss formed from ``hidden_states`` gets none. Each layer then also
-        keeps its last forward's ``expert_counts``."""
+        returns (0: off); a loss formed from ``hidden_states`` gets none. Tokens that a loss's
+        ``valid`` (bool, one per token) leaves out, such as padding, do not count in it. Each
+        layer then also keeps its last forward's ``expert_counts``."""
         if not coef >= 0.0:
             raise ValueError(f"the balance loss's coefficient must be >= 0, not {coef}")
         self.balance_coef = float(coef)
         for layer in self.layers:
             layer.balance = coef > 0.0
 
-    def _hidden(self, input_ids, pos):
+    def _hidden(self, input_ids, pos, valid=None):
         """Hidden states of one token stream, and the layers' balance losses (none without
         gradients, or where the loss is off)."""
         x = F.embedding(input_ids.view(-1), self.embed)
+        valid = None if valid is None else valid.reshape(-1)
         balance = []
         for layer in self.layers:
-            x = layer(x, pos)
+            x = layer(x, pos, valid)
             if layer.balance_loss is not None:
                 balance.append(layer.balance_loss)
                 layer.balance_loss = None  # its graph lives as long as the loss's
@@ -160,25 +162,29 @@ class Qwen3MoeForCausalLM(nn.Module):
     def hidden_states(self, input_ids, pos=None):
         return self._hidden(input_ids, pos)[0]
 
-    def forward(self, input_ids, labels=None, num_valid=None, pos=None):
-        h, balance = self._hidden(input_ids, pos)
+    def forward(self, input_ids, labels=None, num_valid=None, pos=None, valid=None):
+        h, balance = self._hidden(input_ids, pos, valid)
         if labels is None:
             return dense_fwd(h, self.lm_head)
         return self._with_balance(lm_head_xent(h, self.lm_head, labels.view(-1), num_valid), balance)
 
-    def distill(self, input_ids, teacher_ids, teacher_logits, temperature=1.0, num_valid=None, pos=None):
+    def distill(self, input_ids, teacher_ids, teacher_logits, temperature=1.0, num_valid=None, pos=None,
+                valid=None):
         """Distillation loss of one token stream from a teacher's top logits ``[T, K]`` per
         token (see ``spec_ep.ops.loss.topk_distill_loss``)."""
-        h, balance = self._hidden(input_ids, pos)
-        return self._with_balance(lm_head_distill(h, self.lm_head, teacher_ids, teacher_logits, temperature, num_valid),
-                                  balance)
+        h, balance = self._hidden(input_ids, pos, valid)
+        ids, t = (x.reshape(-1, x.shape[-1]) for x in (teacher_ids, teacher_logits))
+        return self._with_balance(lm_head_distill(h, self.lm_head, ids, t, temperature, num_valid), balance)
 
-    def policy(self, input_ids, actions, old_logp, advantages, ref_logp=None, pos=None, **kw) -> PolicyLoss:
+    def policy(self, input_ids, actions, old_logp, advantages, ref_logp=None, pos=None, valid=None,
+               **kw) -> PolicyLoss:
         """Clipped policy loss of one token stream: ``actions[t]`` is the token chosen after
         token ``t``, -1 where none was (see ``spec_ep.ops.loss.clipped_policy_loss``, whose
         other arguments go through ``kw``)."""
-        h, balance = self._hidden(input_ids, pos)
-        out = lm_head_policy(h, self.lm_head, actions.view(-1), old_logp, advantages, ref_logp, **kw)
+        h, balance = self._hidden(input_ids, pos, valid)
+        actions, old_logp, advantages, ref_logp = (None if x is None else x.reshape(-1)
+                                                   for x in (actions, old_logp, advantages, ref_logp))
+        out = lm_head_policy(h, self.lm_head, actions, old_logp, advantages, ref_logp, **kw)
         return out._replace(loss=self._with_balance(out.loss, balance))
 
     def preference(self, sequences, labels, ref_logp, beta=0.1, label_smoothing=0.0) -> PreferenceLoss:
