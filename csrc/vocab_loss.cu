@@ -262,6 +262,18 @@ struct Expo {
   }
 };
 
+// Sets an element of a vector to -infinity: it adds nothing to a sum.
+template <typename T>
+__device__ __forceinline__ void blank(uint4& v, int element) {
+  const uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;
+  const int at = element * (int)sizeof(T), shift = (at % 4) * 8;
+  const uint32_t mask = sizeof(T) == 4 ? 0xffffffffu : 0xffffu << shift;
+  auto put = [&](uint32_t& w, int i) { w = at / 4 == i ? (w & ~mask) | (none << shift) : w; };
+  put(v.x, 0);
+  put(v.y, 1);
+  put(v.z, 2);
+  put(v.w, 3);
+}
 // Largest element of a vector and ref; NaN gives way.
 template <typename T>
 __device__ __forceinline__ float max_of(const uint4& raw, float ref) {
@@ -276,16 +288,20 @@ __device__ __forceinline__ float max_of(const uint4& raw, float ref) {
 // and 1 - q = rest / (own + rest) keep their digits where q is near 1, and ln q is never above 0.
 //
 // The other terms are formed 2^kShift smaller, so that their arguments stay below 0 for values
-// up to 6.9 tau above the reference (beyond, the reference moves): there the hardware
+// up to 20 tau above the reference (beyond, the reference moves): there the hardware
 // exponential's mean error is one number (measured: -5.0e-8 relative over [-9, 0), -5.1e-8 down
 // to -25; +3.3e-8 above 0), which is taken out of each row's sum in 64 bits. Left in, it adds up
 // over a sequence's tokens while the other errors average out. It is a mean over arguments with
 // spread fractions: in a row of equal logits (or at a temperature that makes them equal) it may
-// itself be the error, below half a rounding of the row's log-probability.
-constexpr float kShift = 10.f, kShiftUp = 1024.f;
-// What a thread's sum of shifted terms may grow to before its reference moves. A thread has at
-// most kMaxSlots * 16 terms of a row, in the present shapes 208, so terms near the reference
-// stay below 208 * 2^(0.5 - kShift) = 0.29; one with an argument above 0 does not.
+// itself be the error, below half a rounding of the row's log-probability. A shift of 10 moves
+// the reference of rows with a few large logits: 576 instead of 493 us for 4096 x 151936 with 30
+// logits of 8 to 20 in each row. An argument near -30 is rounded by 2^-20: where a few terms
+// have a row's weight they lie above the reference, with smaller arguments; where many have it,
+// their roundings average out.
+constexpr float kShift = 30.f, kShiftUp = 1073741824.f;
+// What a thread's sum of shifted terms may grow to before its reference moves: 512 terms (what a
+// ring of kMaxSlots holds for a thread) near the reference are below 2^(9.5 - kShift); one with
+// an argument above 0 is not below 1.
 constexpr float kMostSum = 1.f;
 constexpr double kExpMeanError = -5.05e-8;
 // What the fast form z c2 + R adds for reference m: NaN (or infinity) where the sum has to
@@ -311,20 +327,6 @@ __device__ __noinline__ float2 careful_sum(const uint4* v, int n, int step, C2 c
     for (int i = 0; i < Elem<T>::N; ++i) sum += ex2(w.arg(o[i]) - kShift);
   }
   return make_float2(m, sum);
-}
-// Sets an element of a vector to -infinity: it adds nothing to the sum.
-template <typename T>
-__device__ __noinline__ void blank(uint4* v, int element) {
-  const uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;
-  const int at = element * (int)sizeof(T), shift = (at % 4) * 8;
-  const uint32_t mask = sizeof(T) == 4 ? 0xffffffffu : 0xffffu << shift;
-  uint4 o = *v;
-  auto put = [&](uint32_t& w, int i) { w = at / 4 == i ? (w & ~mask) | (none << shift) : w; };
-  put(o.x, 0);
-  put(o.y, 1);
-  put(o.z, 2);
-  put(o.w, 3);
-  *v = o;
 }
 template <typename T>
 __device__ __noinline__ void careful_store(const uint4* v, T* row, int V, int64_t e0, C2 c2, float m, float As) {
@@ -658,8 +660,8 @@ __global__ void __launch_bounds__(512) vocab_row_kernel(const VocabLossArgs a) {
 // which frees them for the next row. So every logit is read from memory once, and loads,
 // arithmetic and stores of neighbouring rows overlap.
 //   first CW warps  sum and gradient: thread i owns vectors i, i + 32 CW, .. of every piece
-//   load warp       bulk copies of whole vectors; the partial vectors at a row's ends come
-//                   from the prepare warp
+//   load warp       bulk copies of whole vectors; the partial vectors at a row's ends, and the
+//                   token's without the token, come from the prepare warp
 //   prepare warp    tokens (8 rows at a time) or teacher entries of the rows to come
 //   join warp       the row's sum from all warps' parts and the factor of its gradient;
 //                   distillation: the gradient at the entries' ids, once the block's dense part
@@ -697,7 +699,9 @@ struct StreamShared {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
   uint64_t ent_full[kTokens], ent_done[kTokens], dense_done[kTokens];
   uint64_t pairs_full[2], factor_full[2];
-  uint4 edge[kTokens][2];  // a row's first and last vector, where they are partial
+  // a row's first and last vector, where they are partial, and the token's, where it is neither
+  // of those; without the token
+  uint4 edge[kTokens][3];
   Token token[kTokens];
   float factor[2][4];  // A, A / sum, reference, sum without the token
   float2 pairs[2][kMaxCluster * kMaxConsumers];
@@ -773,6 +777,17 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
     *j0 = min(rank * per, z.nv);
     *j1 = min(*j0 + per, z.nv);
   };
+  // the vector that an element is in
+  auto vec_of = [](const RowVec<T>& z, int id) { return (int)(((int64_t)id + z.a) / N); };
+  // edge i of entry e: a row's first or last vector, if partial, or the token's, without the token
+  auto prepare_vec = [&](const RowVec<T>& z, int id, int e, int i) {
+    const int own = id >= 0 ? vec_of(z, id) : -1;
+    const int j = i == 0 ? 0 : i == 1 ? z.nv - 1 : own;
+    if (j < 0 || z.full(j) != (i == 2)) return;
+    uint4 v = z.load(j);
+    if (j == own) blank<T>(v, (int)(((int64_t)id + z.a) % N));
+    sh.edge[e][i] = v;
+  };
   // position in the ring of rows: entry e, in its lap's phase
   auto next_entry = [&](int& e, int& lap) {
     if (++e == rows_ahead) {
@@ -792,6 +807,7 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
         int j0, j1;
         part(z, &j0, &j1);
         const int f0 = z.full(0) ? 0 : 1, f1 = z.full(z.nv - 1) ? z.nv : z.nv - 1;  // whole vectors
+        const int id = sh.token[e].id, own = id >= 0 ? vec_of(z, id) : -1;
         for (int p = j0; p < j1; p += kPieceVecs) {
           const int q = min(p + kPieceVecs, j1);
           if (!wait(&sh.empty[slot], turn ^ 1)) { ok = false; break; }
@@ -800,11 +816,16 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
             const bool head = p < f0, tail = q > f1;
             if (head) dst[0] = sh.edge[e][0];
             if (tail && z.nv - 1 >= f0) dst[z.nv - 1 - p] = sh.edge[e][1];
-            if (head || tail) fence_proxy_async_smem();  // before a later bulk copy into the slot
             const int b0 = max(p, f0), b1 = min(q, f1);
-            if (b1 > b0) {
-              mbar_arrive_expect_tx(&sh.full[slot], (uint32_t)(b1 - b0) * 16u);
-              bulk_load(dst + (b0 - p), z.p + z.first(b0), (uint32_t)(b1 - b0) * 16u, &sh.full[slot]);
+            const bool cut = own >= b0 && own < b1;
+            if (cut) dst[own - p] = sh.edge[e][2];
+            if (head || tail || cut) fence_proxy_async_smem();  // before a later bulk copy into the slot
+            const int c0 = cut ? own : b1, c1 = cut ? own + 1 : b1;  // copied: b0 .. c0 and c1 .. b1
+            const int n = b1 - b0 - (cut ? 1 : 0);
+            if (n > 0) {
+              mbar_arrive_expect_tx(&sh.full[slot], (uint32_t)n * 16u);
+              if (c0 > b0) bulk_load(dst + (b0 - p), z.p + z.first(b0), (uint32_t)(c0 - b0) * 16u, &sh.full[slot]);
+              if (b1 > c1) bulk_load(dst + (c1 - p), z.p + z.first(c1), (uint32_t)(b1 - c1) * 16u, &sh.full[slot]);
             } else {
               mbar_arrive(&sh.full[slot]);
             }
@@ -829,14 +850,9 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
         const RowVec<T> z = row_z(t);
         if (t == a.stall_row && rank == 0) break;
         if (!wait(&sh.ent_done[e], lap ^ 1)) break;
-        const bool head = !z.full(0), tail = !z.full(z.nv - 1);
-        if (head || tail) {  // lanes 0..N-1: the first vector, 16..16+N-1: the last
-          const int64_t at = lane < 16 ? z.first(0) + lane : z.first(z.nv - 1) + (lane - 16);
-          const float v = (lane & 15) < N && at >= 0 && at < z.V ? Elem<T>::f(z.p[at]) : -INFINITY;
-          if ((lane & 15) < N) reinterpret_cast<T*>(&sh.edge[e][lane >> 4])[lane & 15] = Elem<T>::t(v);
-        }
         RowRecord r = {};
         const int state = load_entries(a, t, z.p, entries(e), lane, &r);
+        if (state != kRowOff && lane < 3) prepare_vec(z, r.id, e, lane);
         __syncwarp();
         if (lane == 0) {
           sh.token[e].state = state;
@@ -868,10 +884,9 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
         if (mine && !(t == a.stall_row && rank == 0)) {
           const RowVec<T> z = row_z((int)t);
           const Token k = load_token<T, OP>(a, (int)t, z.p);
-          if (k.state != kRowOff) {
-            if (!z.full(0)) sh.edge[e][0] = z.load(0);
-            if (!z.full(z.nv - 1)) sh.edge[e][1] = z.load(z.nv - 1);
-          }
+          if (k.state != kRowOff)
+#pragma unroll
+            for (int i = 0; i < 3; ++i) prepare_vec(z, k.id, e, i);
           sh.token[e] = k;
           if (rank == 0) {
             recs[t].z = k.z;
@@ -958,9 +973,6 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
     // the row that is summed: done of np pieces
     int t = cluster, np = 0, done = 0, part_n = 0;
     bool open = false;
-    // the token that the sum leaves out: its piece (-1: none in this block's part), and its
-    // element within the part where it is this thread's
-    int apart_piece = -1, apart = -1;
     float ref = -INFINITY, sum = 0.f;
     F2 nR2 = f2(0.f, 0.f);
     // the row that waits for its factor
@@ -983,11 +995,6 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
           done = 0;
           ref = -INFINITY;
           sum = 0.f;
-          const int id = sh.token[e].id;
-          const int own = (int)(((int64_t)id + z.a) / N) - j0;
-          const bool here = id >= 0 && own >= 0 && own < part_n;
-          apart_piece = here ? own / kPieceVecs : -1;
-          apart = here && own % Cfg::Lanes == tid ? (int)((int64_t)id + z.a - (int64_t)j0 * N) : -1;
           break;
         }
         if (a.grad) {
@@ -1028,14 +1035,6 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
           const float R = reference(ref, c2);
           nR2 = f2(R, R);
         };
-        // the gradient writes this element by itself
-        auto leave_out = [&](int sl) {
-          if (apart >= 0) {
-            const int at = apart - apart_piece * (kPieceVecs * N);
-            blank<T>(reinterpret_cast<uint4*>(ring + (size_t)sl * kPieceBytes) + at / N, at % N);
-            fence_proxy_async_smem();  // before a later bulk copy into the slot
-          }
-        };
         auto next_slot = [&] {
           if (!a.grad) {
             __syncwarp();
@@ -1065,7 +1064,6 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
               goto out;
             }
             const uint4* piece1 = piece_at(slot1);
-            if ((unsigned)(apart_piece - done) < 2u) leave_out(apart_piece == done ? slot : slot1);
             uint4 raw[2 * Cfg::VPT];
 #pragma unroll
             for (int v = 0; v < Cfg::VPT; ++v) {
@@ -1088,7 +1086,6 @@ __global__ void __launch_bounds__(Cfg::Threads, Cfg::B) vocab_stream_kernel(cons
             continue;
           }
           const int left = (end - tid + Cfg::Lanes - 1) / Cfg::Lanes;  // this thread's vectors (or < 1)
-          if (apart_piece == done) leave_out(slot);
           uint4 raw[Cfg::VPT];
           if (end >= kPieceVecs) {
 #pragma unroll
