@@ -673,14 +673,14 @@ __global__ void __launch_bounds__(512) vocab_row_kernel(const VocabLossArgs a) {
 // gradients among them, and with them the loss, into NaN.
 //
 // What bounds it: memory would take 380 us for 4096 x 151936 bf16 with gradients (2.5 GB at
-// 6.55 TB/s); measured 484-502 us, 5.1 TB/s, with every byte moved once (a capture of 1024
-// rows reads 313 MB and writes 311 MB, the last 55 MB of it still in L2). The two
-// exponentials per logit keep the special-function unit 57% busy and the schedulers 48%: the
+// 6.55 TB/s); measured 490-516 us, 4.8-5.1 TB/s, with every byte moved once (a capture of 1024
+// rows reads 313 MB and writes 311 MB, the last 58 MB of it still in L2). The two
+// exponentials per logit keep the special-function unit 55% busy and the schedulers 49%: the
 // consumers' own latencies (a wait costs ~120 cycles, a row's exchange of sums ~2500, hidden
-// behind the next row's first pieces) set the pace, not memory. The forward alone: 276 us,
-// 4.5 TB/s. Other shapes measured on the same rows: 8 x 4 vectors 545 us, 24 or 28 warps
-// 600-654 us (more waits for the same work), clusters of 4 blocks 990 us with one block and
-// 569 us with two blocks per SM, pieces held in registers instead of the ring 575-641 us.
+// behind the next row's first pieces) set the pace, not memory. The forward alone: 270 us,
+// 4.6 TB/s. Other shapes, measured when these rows took 484-502 us: 8 x 4 vectors 545 us, 24 or
+// 28 warps 600-654 us (more waits for the same work), clusters of 4 blocks 990 us with one block
+// and 569 us with two blocks per SM, pieces held in registers instead of the ring 575-641 us.
 // ------------------------------------------------------------------------------------
 constexpr int kMaxSlots = 32, kMaxCluster = 8, kMaxConsumers = 16;
 
@@ -1544,10 +1544,10 @@ void launch_stream(const VocabLossArgs& a, int C, int rows_ahead, int ent, cudaS
 
 // One block of 16 warps per SM, or more and smaller blocks. What a row costs beside its
 // vectors (waits, the exchange of sums: some 3000 cycles) overlaps between the blocks of an
-// SM, so short rows want many small blocks and long ones the whole ring. Policy loss, us on a
-// B200, for 1 / 2 / 4 / 8 blocks per SM: 4096 x 32001 bf16 146 / 132 / - / -; 16384 x 8000
-// - / 186 / 152 / 149; 16384 x 4096 - / 136 / 100 / 95 (-: the row does not fit, or the next
-// smaller kind already wins).
+// SM, so short rows want many small blocks and long ones the whole ring. Policy loss with its
+// gradient, us on a B200, for 1 / 2 / 4 / 8 blocks per SM: 4096 x 32001 bf16 156 / 137 / - / -;
+// 16384 x 8000 301 / 214 / 167 / -; 16384 x 4096 273 / 161 / 115 / 115; 60000 x 1000
+// 874 / 500 / 295 / 245 (-: the row does not fit).
 using CfgBig = StreamCfg<16, 2, 1>;
 using CfgMid = StreamCfg<8, 2, 2>;
 using CfgSmall = StreamCfg<4, 2, 4>;

@@ -97,7 +97,7 @@ def topk_distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     entries is not in the loss, its logits are not read and its gradient is 0. The same id
     twice counts with both weights. An id outside the vocabulary makes the loss NaN.
     ``num_valid`` (rows with an entry, if the host knows it) spares a count on the device.
-    Gradients reach ``logits`` only.
+    Gradients reach ``logits`` only, once through reverse mode; forward-mode tangents are refused.
     """
     return load().topk_distill(logits, teacher_ids.contiguous(), _f32(teacher_logits), float(temperature),
                                _valid(num_valid))
